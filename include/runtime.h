@@ -306,6 +306,59 @@ int qv_attention_noalloc(float *out, void *key_cache, void *value_cache,
                          const float *q_norm, const float *k_norm,
                          int batch, int position, float epsilon, void *stream);
 
+/* ---- 8-bit serving: e4m3 activations and weights, an int8 K/V cache ----
+ * (no counterpart in the reference).  Device memory, asynchronous on
+ * `stream`, nothing is allocated.  Together they run an attention layer:
+ * qv_norm8 -> qv_mm8 (q and gate, k, v) -> qv_attention8 (with
+ * qv_cache8_pack every 64 tokens) -> qv_quantize8 -> qv_mm8.
+ *
+ * e4m3 codes: [tokens][width] bytes with fp32 scales
+ * [ceil(width/128)][tokens]; a value is code * scale, where a scale belongs
+ * to one token and 128 columns and is that block's largest magnitude / 448.
+ * A block that holds a value which is not finite has the scale NaN and zero
+ * codes.
+ *
+ * qv_norm8: s = x + residual (residual NULL: s = x), y = s *
+ * rsqrt(mean(s^2) + epsilon) * weights, codes and scales of y.  residual_out
+ * (NULL: not written) receives s, normed (NULL: not written) y in fp32; either
+ * may be x or residual itself, and they must not be the same buffer.
+ * x, residual: [tokens][width]; weights: [width]; 1 <= width <= 17408.
+ * qv_quantize8: codes and scales of x itself. */
+int qv_norm8(void *codes, float *scales, float *residual_out, float *normed,
+             const float *x, const float *residual, const float *weights,
+             int tokens, int width, float epsilon, void *stream);
+int qv_quantize8(void *codes, float *scales, const float *x, int tokens, int width,
+                 void *stream);
+
+/* out [tokens][rows] (fp32) = X W^T for e4m3 codes: weights [rows][width] with
+ * fp32 weight_scales [ceil(rows/128)][ceil(width/128)] (one for every block of
+ * 128 x 128), codes [tokens][width] with scales as above.  Any fp32 scales.
+ * width a multiple of 16 up to 65536, 1..248320 rows, tokens 1..139264;
+ * weights and codes 16-byte aligned. */
+int qv_mm8(float *out, const void *weights, const float *weight_scales,
+           const void *codes, const float *scales, int tokens, int width, int rows,
+           void *stream);
+
+/* int8 K/V cache: codes [blocks][4][64][256] (16-byte aligned) and fp32
+ * scales [blocks][4] for K and for V, where block b holds the positions
+ * [64 b, 64 b + 64); a value is code * scale, scale = largest magnitude / 127
+ * over the block's 64 rows of the head, code = the value / scale rounded to the
+ * nearest integer (ties to even).  A block and head that holds a value which
+ * is not finite has the scale NaN.
+ *
+ * qv_cache8_pack writes the blocks of positions [begin, end) (multiples of 64,
+ * end <= 139264) from fp16 rows [ring_rows][4][256]; position r is row r %
+ * ring_rows.  ring_rows >= end (a plain cache), or a multiple of 64 that is at
+ * least end - begin (the tail of qv_attention8).
+ * qv_cache8_unpack writes positions [begin, end) as fp16 rows, the position
+ * `begin` at row 0. */
+int qv_cache8_pack(void *key_codes, float *key_scales, void *value_codes, float *value_scales,
+                   const void *key_rows, const void *value_rows, int begin, int end,
+                   int ring_rows, void *stream);
+int qv_cache8_unpack(void *key_rows, void *value_rows, const void *key_codes,
+                     const float *key_scales, const void *value_codes,
+                     const float *value_scales, int begin, int end, void *stream);
+
 /* Synchronise the current device and return (then clear) the status word
  * that kernels set when a bounded internal wait gives up: 0 = none. */
 int qv_status(void);

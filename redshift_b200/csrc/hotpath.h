@@ -77,6 +77,23 @@ void delta_prefill(float *out, float *state, float *history, const float *qkv, c
                    const float *beta, const float *conv, const float *decay, const float *bias, const float *norm, int T,
                    int Hk, int Hv, int D, float eps, void *ws, size_t ws_bytes, cudaStream_t st);
 
+// 8-bit serving (quant8.cu): the K/V cache in int8 with a scale for every
+// CACHE8_BLOCK tokens and head, codes [block][4][64][256]; rows [begin, end),
+// begin and end block borders for packing, source row r at r % ring.
+constexpr int CACHE8_BLOCK = 64;
+void cache8_pack(int8_t *kc, float *ks, int8_t *vc, float *vs, const __half *k, const __half *v, int begin, int end,
+                 int ring, cudaStream_t st);
+void cache8_unpack(__half *k, __half *v, const int8_t *kc, const float *ks, const int8_t *vc, const float *vs, int begin,
+                   int end, cudaStream_t st);
+// e4m3 codes [tokens][width] with scales [ceil(width/128)][tokens] of x, or with
+// weights of the RMSNorm of x (+ residual); sum_out, normed and residual may be null.
+void norm8(uint8_t *codes, float *scales, float *sum_out, float *normed, const float *x, const float *residual,
+           const float *weights, int tokens, int width, float eps, cudaStream_t st);
+// Block-scaled e4m3 product (mm8.cu): out [tokens][rows], weights [rows][width]
+// with scales [ceil(rows/128)][ceil(width/128)], x as norm8 writes it.
+void mm8(float *out, const void *weights, const float *weight_scales, const void *x, const float *scales, int tokens,
+         int width, int rows, cudaStream_t st);
+
 // The thread-local message behind qv_error() (runtime.cu).
 void clear_error();
 void record_error(const char *message);

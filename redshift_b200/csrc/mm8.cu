@@ -1,0 +1,511 @@
+// Matrix product of e4m3 codes with block scales (sm_100a tcgen05, kind::f8f6f4):
+//   out[t][r] = sum over blocks b of 128 columns of
+//               weight_scale[r / 128][b] * scale[b][t] * sum_{k in b} W[r][k] X[t][k]
+// for weights W [rows][width], activations X [tokens][width] and fp32 scales.
+//
+// Every block's sum of 128 products leaves the tensor core as fp32 and is
+// multiplied by its two scales and added in fp32 registers, so the scales may
+// be any fp32 values and a long width costs no precision (the products of one
+// block are exact in the accumulator's alignment for codes of like size).
+//
+// Two kernels:
+//  * few_kernel<NT> (tokens as the MMA's N, 16..128 of them): 128 weight rows
+//    per CTA.  Bound by reading the weights once from HBM; the width is split
+//    over a cluster of up to 8 CTAs whose partial sums meet in distributed
+//    shared memory in a fixed order, so that also few rows fill the SMs and no
+//    workspace or atomics are needed.
+//  * many_kernel (128 tokens as the MMA's M, 256 weight rows as its N):
+//    persistent CTAs.  Bound by the tensor pipe; with tokens in the TMEM lanes
+//    the two scales of a thread's columns are one factor per block.
+#include "common.cuh"
+#include "hotpath.h"
+
+#include <algorithm>
+#include <stdexcept>
+#include <string>
+
+namespace qv {
+namespace {
+
+constexpr int KB = 128;                        // columns of a block = one 128-byte swizzled row of codes
+constexpr int ROWS = 128;                      // weight rows that share a scale
+
+// D[tmem] (+)= A[smem] * B[smem]^T for e4m3 codes, fp32 accumulate, K = 32.
+__device__ __forceinline__ void mma_e4m3_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                            uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p;\n\t"
+                 "setp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+                 :: "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate) : "memory");
+}
+// Instruction descriptor: e4m3 operands (format 0 of kind::f8f6f4), both K-major, fp32 accumulator.
+__host__ __device__ constexpr uint32_t idesc_e4m3(int M, int N) {
+    return (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
+}
+// Asynchronous copy of one float into shared memory, zero when !live.
+__device__ __forceinline__ void copy_float(float *dst, const float *src, bool live) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;"
+                 :: "r"(smem_addr(dst)), "l"(src), "r"(live ? 4 : 0) : "memory");
+}
+// Arrive on `bar` (counted in its initial count) once this thread's copies have landed.
+__device__ __forceinline__ void arrive_copies(uint64_t *bar) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" :: "r"(smem_addr(bar)) : "memory");
+}
+__device__ __forceinline__ bool warp_wait8(uint64_t *bar, uint32_t parity, volatile int *abort_flag) {
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag));
+}
+__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+struct Mm8Params {
+    float *out;
+    const float *weight_scales, *scales;
+    int tokens, rows, blocks;                  // blocks = ceil(width / 128)
+    int splits;                                // cluster size (few_kernel)
+    int m_tiles, tiles;                        // many_kernel: token tiles, all tiles
+};
+
+// ---------------------------------------------------------------- few tokens
+template <int NT> struct Few {
+    // Two CTAs per SM up to 64 tokens (their rings hold 2 x 90..108 KB in
+    // flight, enough for the HBM latency), one at 128.
+    static constexpr int STAGES = NT == 16 ? 6 : NT == 32 ? 5 : NT == 64 ? 4 : 6;
+    static constexpr int BUFS = NT <= 32 ? 4 : 2;            // TMEM accumulators
+    static constexpr int CTAS = NT <= 64 ? 2 : 1;
+    static constexpr int SLOTS = STAGES + BUFS;              // scale slots
+    static constexpr int W_BYTES = ROWS * KB, X_BYTES = NT * KB, STAGE = W_BYTES + X_BYTES;
+    static constexpr int SLOT_FLOATS = NT + 4;
+    static constexpr int SM_SCALE = STAGES * STAGE;
+    static constexpr int SM_BAR = SM_SCALE + SLOTS * SLOT_FLOATS * 4;
+    static constexpr int SMEM = SM_BAR + 256;
+    static_assert(NT * ROWS * 4 <= STAGES * STAGE, "partial sums exceed the ring");
+    static_assert((2 * STAGES + 2 * BUFS + SLOTS + 1) * 8 + 8 <= 256, "barrier area");
+};
+
+template <int NT>
+__global__ void __launch_bounds__(192, Few<NT>::CTAS)
+few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX, const Mm8Params p) {
+    using L = Few<NT>;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    uint64_t *full = reinterpret_cast<uint64_t *>(smem + L::SM_BAR), *empty = full + L::STAGES;
+    uint64_t *d_full = empty + L::STAGES, *d_empty = d_full + L::BUFS, *s_full = d_empty + L::BUFS;
+    uint64_t *mma_done = s_full + L::SLOTS;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(mma_done + 1);
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
+    float *slots = reinterpret_cast<float *>(smem + L::SM_SCALE);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int split = blockIdx.x, rtile = blockIdx.y, t0 = blockIdx.z * NT;
+    const int b0 = (int)((long long)p.blocks * split / p.splits), b1 = (int)((long long)p.blocks * (split + 1) / p.splits);
+    const int n = b1 - b0;
+    const bool bad_base = (smem_addr(smem) & 1023) != 0;      // 128B-swizzle atoms need a 1024-byte aligned base
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < L::STAGES; ++i) { mbar_init(full + i, 1); mbar_init(empty + i, 1); }
+        for (int i = 0; i < L::BUFS; ++i) { mbar_init(d_full + i, 1); mbar_init(d_empty + i, 4); }
+        for (int i = 0; i < L::SLOTS; ++i) mbar_init(s_full + i, 32);
+        mbar_init(mma_done, 1);
+        *abort_flag = bad_base ? 1 : 0;
+        if (bad_base) raise_status(STATUS_BAD_ARGUMENT);
+        fence_barrier_init();
+        prefetch_tmap(&tmW);
+        prefetch_tmap(&tmX);
+    }
+    if (warp == 1) { tmem_alloc(tmem_slot, L::BUFS * NT); tmem_relinquish(); }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    grid_dependency_wait();
+    if (threadIdx.x == 0) launch_dependents();
+
+    float acc[NT];
+#pragma unroll
+    for (int c = 0; c < NT; ++c) acc[c] = 0.f;
+    bool ok = !bad_base;
+    if (warp == 0) {
+        // ------------------------------------------------ producer: code tiles by TMA, scales by small copies
+        int issued = 0;
+        for (int j = 0; j < n && ok; ++j) {
+            const int s = j % L::STAGES, slot = j % L::SLOTS, b = b0 + j;
+            if (j >= L::STAGES && !warp_wait8(empty + s, (j / L::STAGES - 1) & 1, abort_flag)) { ok = false; break; }
+            if (lane == 0) {
+                uint8_t *w = smem + s * L::STAGE;
+                mbar_expect_tx(full + s, L::STAGE);
+                tma_load_2d(w, &tmW, full + s, b * KB, rtile * ROWS);
+                tma_load_2d(w + L::W_BYTES, &tmX, full + s, b * KB, t0);
+            }
+            issued = j + 1;
+            // A slot is free again here: the MMA of block j - STAGES has run,
+            // which waited until block j - SLOTS had left its accumulator.
+            float *d = slots + slot * L::SLOT_FLOATS;
+            for (int t = lane; t < NT; t += 32) {
+                const bool live = t0 + t < p.tokens;
+                copy_float(d + t, p.scales + (size_t)b * p.tokens + (live ? t0 + t : 0), live);
+            }
+            if (lane == 0) copy_float(d + NT, p.weight_scales + (size_t)rtile * p.blocks + b, true);
+            arrive_copies(s_full + slot);
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        // Every issued load must land before the CTA may exit or reuse the ring.
+        if (lane == 0) {
+            const long long start = clock64();
+            for (int j = max(0, issued - L::STAGES); j < issued; ++j)
+                while (!mbar_try_wait(full + j % L::STAGES, (j / L::STAGES) & 1) && clock64() - start < WAIT_LIMIT_CYCLES) {}
+        }
+    } else if (warp == 1) {
+        // ------------------------------------------------ MMA issuer
+        if (lane == 0) {
+            constexpr uint32_t idesc = idesc_e4m3(ROWS, NT);
+            for (int j = 0; j < n && ok; ++j) {
+                const int s = j % L::STAGES, d = j % L::BUFS;
+                if (!mbar_wait(full + s, (j / L::STAGES) & 1, abort_flag)) { ok = false; break; }
+                if (j >= L::BUFS && !mbar_wait(d_empty + d, (j / L::BUFS - 1) & 1, abort_flag)) { ok = false; break; }
+                tc_fence_after();
+                const uint32_t w = smem_addr(smem + s * L::STAGE), x = w + L::W_BYTES;
+#pragma unroll
+                for (int k = 0; k < KB / 32; ++k)
+                    mma_e4m3_ss(tmem + d * NT, sw128_desc(w + k * 32, 16, 1024), sw128_desc(x + k * 32, 16, 1024), idesc,
+                                k > 0 ? 1u : 0u);
+                mma_commit(empty + s);
+                mma_commit(d_full + d);
+            }
+            mma_commit(mma_done);
+            const long long start = clock64();
+            while (!mbar_try_wait(mma_done, 0) && clock64() - start < WAIT_LIMIT_CYCLES) {}
+        }
+    } else {
+        // ------------------------------------------------ scales and sums: thread = TMEM lane = weight row
+        const uint32_t t_lane = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+        for (int j = 0; j < n; ++j) {
+            const int d = j % L::BUFS, slot = j % L::SLOTS;
+            if (!warp_wait8(s_full + slot, (j / L::SLOTS) & 1, abort_flag) ||
+                !warp_wait8(d_full + d, (j / L::BUFS) & 1, abort_flag)) { ok = false; break; }
+            tc_fence_after();
+            const float *sc = slots + slot * L::SLOT_FLOATS;
+            const float ws = sc[NT];
+#pragma unroll
+            for (int c0 = 0; c0 < NT; c0 += 16) {
+                float x[16];
+                tmem_ld16(t_lane + d * NT + c0, x);
+                tmem_wait_ld();
+#pragma unroll
+                for (int c = 0; c < 16; c += 4) {
+                    const float4 f = *reinterpret_cast<const float4 *>(sc + c0 + c);
+                    acc[c0 + c] = fmaf(x[c], f.x * ws, acc[c0 + c]);
+                    acc[c0 + c + 1] = fmaf(x[c + 1], f.y * ws, acc[c0 + c + 1]);
+                    acc[c0 + c + 2] = fmaf(x[c + 2], f.z * ws, acc[c0 + c + 2]);
+                    acc[c0 + c + 3] = fmaf(x[c + 3], f.w * ws, acc[c0 + c + 3]);
+                }
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(d_empty + d);
+        }
+    }
+    __syncwarp();
+    tc_fence_before();
+    const int all_ok = __syncthreads_and(ok);
+    tc_fence_after();
+    if (warp == 1) tmem_dealloc(tmem, L::BUFS * NT);
+
+    const int lrow = (warp & 3) * 32 + lane, row = rtile * ROWS + lrow;
+    const int live = min(NT, p.tokens - t0);
+    if (p.splits == 1) {
+        if (warp >= 2 && all_ok && row < p.rows) {
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+                if (t < live) p.out[(size_t)(t0 + t) * p.rows + row] = acc[t];
+        }
+        return;
+    }
+    // Partial sums of the splits meet in shared memory (the idle ring); CTA q
+    // of the cluster adds the tokens q, q + splits, ... in the order of the
+    // splits.  Every CTA of the cluster passes both barriers.
+    float *part = reinterpret_cast<float *>(smem);
+    int *good = reinterpret_cast<int *>(slots);               // this CTA's partial sums are complete
+    if (warp >= 2) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t) part[t * ROWS + lrow] = acc[t];
+    }
+    if (threadIdx.x == 0) *good = all_ok;
+    cluster_sync();
+    if (warp >= 2 && row < p.rows) {
+        bool fine = true;
+        for (int q = 0; q < p.splits; ++q) fine = fine && __float_as_int(ld_cluster_f32(cluster_map(good, q))) != 0;
+        for (int t = split; fine && t < live; t += p.splits) {
+            float v = 0.f;
+            for (int q = 0; q < p.splits; ++q) v += ld_cluster_f32(cluster_map(part + t * ROWS + lrow, q));
+            p.out[(size_t)(t0 + t) * p.rows + row] = v;
+        }
+    }
+    cluster_sync();
+}
+
+// ---------------------------------------------------------------- many tokens
+struct Many {
+    static constexpr int MT = 128, NT = 256;                 // tokens, weight rows of a tile
+    static constexpr int STAGES = 4, BUFS = 2, SLOTS = STAGES + BUFS;
+    static constexpr int X_BYTES = MT * KB, W_BYTES = NT * KB, STAGE = X_BYTES + W_BYTES;
+    static constexpr int SLOT_FLOATS = MT + 4;
+    static constexpr int OUT_ROW = 20;                       // floats of a staged row: 16 columns and a pad
+    static constexpr int SM_OUT = STAGES * STAGE;            // [8 warps][32 rows][OUT_ROW]
+    static constexpr int SM_SCALE = SM_OUT + 8 * 32 * OUT_ROW * 4;
+    static constexpr int SM_BAR = SM_SCALE + SLOTS * SLOT_FLOATS * 4;
+    static constexpr int SMEM = SM_BAR + 256;
+    static_assert(SMEM <= 227 * 1024, "shared memory of a CTA");
+};
+
+__global__ void __launch_bounds__(320, 1)
+many_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX, const Mm8Params p) {
+    using L = Many;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    uint64_t *full = reinterpret_cast<uint64_t *>(smem + L::SM_BAR), *empty = full + L::STAGES;
+    uint64_t *d_full = empty + L::STAGES, *d_empty = d_full + L::BUFS, *s_full = d_empty + L::BUFS;
+    uint64_t *mma_done = s_full + L::SLOTS;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(mma_done + 1);
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
+    float *slots = reinterpret_cast<float *>(smem + L::SM_SCALE);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const bool bad_base = (smem_addr(smem) & 1023) != 0;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < L::STAGES; ++i) { mbar_init(full + i, 1); mbar_init(empty + i, 1); }
+        for (int i = 0; i < L::BUFS; ++i) { mbar_init(d_full + i, 1); mbar_init(d_empty + i, 8); }
+        for (int i = 0; i < L::SLOTS; ++i) mbar_init(s_full + i, 32);
+        mbar_init(mma_done, 1);
+        *abort_flag = bad_base ? 1 : 0;
+        if (bad_base) raise_status(STATUS_BAD_ARGUMENT);
+        fence_barrier_init();
+        prefetch_tmap(&tmW);
+        prefetch_tmap(&tmX);
+    }
+    if (warp == 1) { tmem_alloc(tmem_slot, 512); tmem_relinquish(); }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    grid_dependency_wait();
+    if (threadIdx.x == 0) launch_dependents();
+
+    // Tiles in order of the token tile first: the CTAs that run together share
+    // a few weight tiles and all of X in L2.
+    const int mine = p.tiles > (int)blockIdx.x ? (p.tiles - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x : 0;
+    const int row_blocks = (p.rows + ROWS - 1) / ROWS;
+    if (bad_base) {
+    } else if (warp == 0) {
+        int j = 0;                                           // blocks since the start, over all tiles
+        bool ok = true;
+        for (int i = 0; i < mine && ok; ++i) {
+            const int tile = blockIdx.x + i * gridDim.x, m0 = tile % p.m_tiles * L::MT, n0 = tile / p.m_tiles * L::NT;
+            for (int b = 0; b < p.blocks; ++b, ++j) {
+                const int s = j % L::STAGES, slot = j % L::SLOTS;
+                if (j >= L::STAGES && !warp_wait8(empty + s, (j / L::STAGES - 1) & 1, abort_flag)) { ok = false; break; }
+                if (lane == 0) {
+                    uint8_t *x = smem + s * L::STAGE;
+                    mbar_expect_tx(full + s, L::STAGE);
+                    tma_load_2d(x, &tmX, full + s, b * KB, m0);
+                    tma_load_2d(x + L::X_BYTES, &tmW, full + s, b * KB, n0);
+                }
+                float *d = slots + slot * L::SLOT_FLOATS;
+#pragma unroll
+                for (int t = 0; t < L::MT; t += 32) {
+                    const bool live = m0 + t + lane < p.tokens;
+                    copy_float(d + t + lane, p.scales + (size_t)b * p.tokens + (live ? m0 + t + lane : 0), live);
+                }
+                if (lane < 2) {
+                    const int rb = n0 / ROWS + lane;
+                    const bool live = rb < row_blocks;
+                    copy_float(d + L::MT + lane, p.weight_scales + (size_t)(live ? rb : 0) * p.blocks + b, live);
+                }
+                arrive_copies(s_full + slot);
+            }
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        if (lane == 0) {
+            const long long start = clock64();
+            for (int q = max(0, j - L::STAGES); q < j; ++q)
+                while (!mbar_try_wait(full + q % L::STAGES, (q / L::STAGES) & 1) && clock64() - start < WAIT_LIMIT_CYCLES) {}
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            constexpr uint32_t idesc = idesc_e4m3(L::MT, L::NT);
+            const int n = mine * p.blocks;
+            for (int j = 0; j < n; ++j) {
+                const int s = j % L::STAGES, d = j % L::BUFS;
+                if (!mbar_wait(full + s, (j / L::STAGES) & 1, abort_flag)) break;
+                if (j >= L::BUFS && !mbar_wait(d_empty + d, (j / L::BUFS - 1) & 1, abort_flag)) break;
+                tc_fence_after();
+                const uint32_t x = smem_addr(smem + s * L::STAGE), w = x + L::X_BYTES;
+#pragma unroll
+                for (int k = 0; k < KB / 32; ++k)
+                    mma_e4m3_ss(tmem + d * L::NT, sw128_desc(x + k * 32, 16, 1024), sw128_desc(w + k * 32, 16, 1024), idesc,
+                                k > 0 ? 1u : 0u);
+                mma_commit(empty + s);
+                mma_commit(d_full + d);
+            }
+            mma_commit(mma_done);
+            const long long start = clock64();
+            while (!mbar_try_wait(mma_done, 0) && clock64() - start < WAIT_LIMIT_CYCLES) {}
+        }
+    } else {
+        // Warps 2-5 take the tile's columns [0, 128), warps 6-9 [128, 256);
+        // thread = TMEM lane = token.
+        const int half = (warp - 2) >> 2, lrow = (warp & 3) * 32;
+        const uint32_t t_col = tmem + ((uint32_t)lrow << 16) + half * 128;
+        float *stage = reinterpret_cast<float *>(smem + L::SM_OUT) + (warp - 2) * 32 * L::OUT_ROW;
+        int j = 0;
+        bool ok = true;
+        for (int i = 0; i < mine && ok; ++i) {
+            const int tile = blockIdx.x + i * gridDim.x, m0 = tile % p.m_tiles * L::MT, n0 = tile / p.m_tiles * L::NT;
+            float2 acc[64];
+#pragma unroll
+            for (int c = 0; c < 64; ++c) acc[c] = make_float2(0.f, 0.f);
+            for (int b = 0; b < p.blocks; ++b, ++j) {
+                const int d = j % L::BUFS, slot = j % L::SLOTS;
+                if (!warp_wait8(s_full + slot, (j / L::SLOTS) & 1, abort_flag) ||
+                    !warp_wait8(d_full + d, (j / L::BUFS) & 1, abort_flag)) { ok = false; break; }
+                tc_fence_after();
+                const float *sc = slots + slot * L::SLOT_FLOATS;
+                const float f = sc[lrow + lane] * sc[L::MT + half];
+                const float2 f2 = make_float2(f, f);
+#pragma unroll
+                for (int c0 = 0; c0 < 128; c0 += 32) {
+                    float x[2][16];
+                    tmem_ld16(t_col + d * L::NT + c0, x[0]);
+                    tmem_ld16(t_col + d * L::NT + c0 + 16, x[1]);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int q = 0; q < 2; ++q)
+#pragma unroll
+                        for (int c = 0; c < 8; ++c)
+                            acc[c0 / 2 + q * 8 + c] = ffma2(make_float2(x[q][2 * c], x[q][2 * c + 1]), f2, acc[c0 / 2 + q * 8 + c]);
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(d_empty + d);
+            }
+            if (!ok) break;
+            // 16 columns at a time through shared memory: 64-byte pieces of eight rows per store.
+            const bool vec = p.rows % 4 == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15) == 0;
+#pragma unroll
+            for (int c0 = 0; c0 < 128; c0 += 16) {
+#pragma unroll
+                for (int c = 0; c < 16; c += 4) {
+                    const float2 a = acc[(c0 + c) / 2], e = acc[(c0 + c) / 2 + 1];
+                    *reinterpret_cast<float4 *>(stage + lane * L::OUT_ROW + c) = make_float4(a.x, a.y, e.x, e.y);
+                }
+                __syncwarp();
+                const int col = n0 + half * 128 + c0 + (lane & 3) * 4;
+#pragma unroll
+                for (int r0 = 0; r0 < 32; r0 += 8) {
+                    const int r = r0 + (lane >> 2), token = m0 + lrow + r;
+                    const float4 v = *reinterpret_cast<const float4 *>(stage + r * L::OUT_ROW + (lane & 3) * 4);
+                    if (token >= p.tokens) continue;
+                    float *dst = p.out + (size_t)token * p.rows + col;
+                    if (vec) {
+                        if (col < p.rows) *reinterpret_cast<float4 *>(dst) = v;
+                    } else {
+                        if (col < p.rows) dst[0] = v.x;
+                        if (col + 1 < p.rows) dst[1] = v.y;
+                        if (col + 2 < p.rows) dst[2] = v.z;
+                        if (col + 3 < p.rows) dst[3] = v.w;
+                    }
+                }
+                __syncwarp();
+            }
+        }
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 1) tmem_dealloc(tmem, 512);
+}
+
+// ---------------------------------------------------------------- host
+// Map over [count][width] codes: box = 128 columns x `box_rows`, 128B swizzle; past the edges zeros are read.
+CUtensorMap codes_map(const void *base, int width, int count, int box_rows) {
+    CUtensorMap m;
+    cuuint64_t dims[2] = {(cuuint64_t)width, (cuuint64_t)count};
+    cuuint64_t strides[1] = {(cuuint64_t)width};
+    cuuint32_t box[2] = {KB, (cuuint32_t)box_rows};
+    cuuint32_t estr[2] = {1, 1};
+    const CUresult r = tensor_map_encoder()(&m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void *>(base), dims, strides,
+                                            box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                                            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) throw std::runtime_error("cuTensorMapEncodeTiled failed: " + std::to_string((int)r));
+    return m;
+}
+
+PerDeviceOnce g_configured;
+template <class K> void reserve(K *kernel, int bytes) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess)
+        throw std::runtime_error("cannot reserve shared memory for the e4m3 product");
+}
+
+template <int NT> void launch_few(Mm8Params p, const void *weights, const void *x, int width, cudaStream_t st) {
+    using L = Few<NT>;
+    const int row_tiles = (p.rows + ROWS - 1) / ROWS, token_tiles = (p.tokens + NT - 1) / NT;
+    // Split the width while the CTAs still fit the SMs at once and every CTA keeps four blocks or more.
+    const long long slots = 148LL * L::CTAS, tiles = (long long)row_tiles * token_tiles;
+    int splits = 1;
+    while (splits < 8 && tiles * splits * 2 <= slots && p.blocks >= 8 * splits) splits *= 2;
+    p.splits = splits;
+    const CUtensorMap mw = codes_map(weights, width, p.rows, ROWS), mx = codes_map(x, width, p.tokens, NT);
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(splits, row_tiles, token_tiles);
+    cfg.blockDim = dim3(192);
+    cfg.dynamicSmemBytes = L::SMEM;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = splits;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, few_kernel<NT>, mw, mx, p);
+    if (e != cudaSuccess) throw std::runtime_error(std::string("e4m3 product: ") + cudaGetErrorString(e));
+}
+
+}  // namespace
+
+void mm8(float *out, const void *weights, const float *weight_scales, const void *x, const float *scales, int tokens,
+         int width, int rows, cudaStream_t st) {
+    g_configured.run([] {
+        reserve(few_kernel<16>, Few<16>::SMEM); reserve(few_kernel<32>, Few<32>::SMEM);
+        reserve(few_kernel<64>, Few<64>::SMEM); reserve(few_kernel<128>, Few<128>::SMEM);
+        reserve(many_kernel, Many::SMEM);
+    });
+    Mm8Params p{out, weight_scales, scales, tokens, rows, (width + KB - 1) / KB, 1, 0, 0};
+    const long long big = (long long)((tokens + Many::MT - 1) / Many::MT) * ((rows + Many::NT - 1) / Many::NT);
+    if (tokens > 128 && big >= 100) {
+        p.m_tiles = (tokens + Many::MT - 1) / Many::MT;
+        p.tiles = (int)big;
+        int dev = 0, sms = 148;
+        if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+        const CUtensorMap mw = codes_map(weights, width, rows, Many::NT), mx = codes_map(x, width, tokens, Many::MT);
+        const cudaError_t e = launch_chained(many_kernel, dim3((unsigned)std::min<long long>(big, sms)), dim3(320), Many::SMEM, st,
+                                             mw, mx, p);
+        if (e != cudaSuccess) throw std::runtime_error(std::string("e4m3 product: ") + cudaGetErrorString(e));
+    } else if (tokens <= 16) {
+        launch_few<16>(p, weights, x, width, st);
+    } else if (tokens <= 32) {
+        launch_few<32>(p, weights, x, width, st);
+    } else if (tokens <= 64) {
+        launch_few<64>(p, weights, x, width, st);
+    } else {
+        launch_few<128>(p, weights, x, width, st);
+    }
+}
+
+}  // namespace qv

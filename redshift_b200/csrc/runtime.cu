@@ -87,6 +87,7 @@ void check_delta_dims(int key_heads, int value_heads, int dim) {
     require((dim == 32 || dim == 128) && key_heads > 0 && value_heads >= key_heads &&
             value_heads <= 48 && value_heads % key_heads == 0, "unsupported DeltaNet dimensions");
 }
+bool aligned16(const void *a) { return (reinterpret_cast<uintptr_t>(a) & 15) == 0; }
 cudaStream_t as_stream(void *s) { return static_cast<cudaStream_t>(s); }
 
 // ------------------------------------------------------------------ attention
@@ -540,6 +541,71 @@ int qv_delta_chunked(float *out, float *state, const void *q, const void *k, con
         qv::delta_chunked(out, state, static_cast<const __half *>(q), static_cast<const __half *>(k),
                           static_cast<const __half *>(v), alpha, beta, decay, bias, tokens, key_heads, value_heads,
                           dim, workspace, workspace_bytes, as_stream(stream));
+    });
+}
+
+// ------------------------------------------------------------------ 8-bit serving
+int qv_cache8_pack(void *key_codes, float *key_scales, void *value_codes, float *value_scales, const void *key_rows,
+                   const void *value_rows, int begin, int end, int ring_rows, void *stream) {
+    return guarded([&] {
+        require(begin >= 0 && begin <= end && end <= kMaxContext && begin % qv::CACHE8_BLOCK == 0 &&
+                end % qv::CACHE8_BLOCK == 0, "packed rows must be whole blocks of 64 within 139264");
+        require(ring_rows >= end || (ring_rows % qv::CACHE8_BLOCK == 0 && ring_rows >= end - begin && ring_rows > 0),
+                "the row buffer neither holds every row nor is a ring of whole blocks that holds the packed ones");
+        require(key_codes && key_scales && value_codes && value_scales && key_rows && value_rows, "null cache buffer");
+        require(aligned16(key_codes) && aligned16(value_codes) && aligned16(key_rows) && aligned16(value_rows),
+                "cache codes and rows must be 16-byte aligned");
+        qv::cache8_pack(static_cast<int8_t *>(key_codes), key_scales, static_cast<int8_t *>(value_codes), value_scales,
+                        static_cast<const __half *>(key_rows), static_cast<const __half *>(value_rows), begin, end,
+                        ring_rows, as_stream(stream));
+    });
+}
+
+int qv_cache8_unpack(void *key_rows, void *value_rows, const void *key_codes, const float *key_scales,
+                     const void *value_codes, const float *value_scales, int begin, int end, void *stream) {
+    return guarded([&] {
+        require(begin >= 0 && begin <= end && end <= kMaxContext, "invalid row range");
+        require(key_codes && key_scales && value_codes && value_scales && key_rows && value_rows, "null cache buffer");
+        require(aligned16(key_codes) && aligned16(value_codes) && aligned16(key_rows) && aligned16(value_rows),
+                "cache codes and rows must be 16-byte aligned");
+        qv::cache8_unpack(static_cast<__half *>(key_rows), static_cast<__half *>(value_rows),
+                          static_cast<const int8_t *>(key_codes), key_scales, static_cast<const int8_t *>(value_codes),
+                          value_scales, begin, end, as_stream(stream));
+    });
+}
+
+int qv_norm8(void *codes, float *scales, float *residual_out, float *normed, const float *x, const float *residual,
+             const float *weights, int tokens, int width, float epsilon, void *stream) {
+    return guarded([&] {
+        require(tokens >= 1 && tokens <= kMaxContext, "tokens must be between 1 and 139264");
+        check_epsilon(epsilon);
+        require(codes && scales && x && weights, "null normalization buffer");
+        require(!residual_out || residual_out != normed, "residual_out and normed must not share a buffer");
+        require(width > 0 && width <= 17408, "invalid normalization width");
+        qv::norm8(static_cast<uint8_t *>(codes), scales, residual_out, normed, x, residual, weights, tokens, width,
+                  epsilon, as_stream(stream));
+    });
+}
+
+int qv_quantize8(void *codes, float *scales, const float *x, int tokens, int width, void *stream) {
+    return guarded([&] {
+        require(tokens >= 1 && tokens <= kMaxContext, "tokens must be between 1 and 139264");
+        require(codes && scales && x, "null quantization buffer");
+        require(width > 0 && width <= 17408, "invalid quantization width");
+        qv::norm8(static_cast<uint8_t *>(codes), scales, nullptr, nullptr, x, nullptr, nullptr, tokens, width, 1.f,
+                  as_stream(stream));
+    });
+}
+
+int qv_mm8(float *out, const void *weights, const float *weight_scales, const void *codes, const float *scales,
+           int tokens, int width, int rows, void *stream) {
+    return guarded([&] {
+        require(tokens >= 1 && tokens <= kMaxContext, "tokens must be between 1 and 139264");
+        require(out && weights && weight_scales && codes && scales, "null projection buffer");
+        require(width >= 16 && width <= 65536 && width % 16 == 0 && rows > 0 && rows <= 248320,
+                "invalid projection dimensions");
+        require(aligned16(weights) && aligned16(codes), "e4m3 codes must be 16-byte aligned");
+        qv::mm8(out, weights, weight_scales, codes, scales, tokens, width, rows, as_stream(stream));
     });
 }
 

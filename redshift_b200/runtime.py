@@ -62,6 +62,11 @@ ADDITIVE_SIGNATURES = {
     'qv_delta_prefill_workspace': ([_I, _I, _I], _S),
     'qv_delta_prefill': ([_P] * 11 + [_I] * 4 + [_F, _P, _S, _P], _I),
     'qv_status': ([], _I),
+    'qv_norm8': ([_P] * 7 + [_I, _I, _F, _P], _I),
+    'qv_quantize8': ([_P] * 3 + [_I, _I, _P], _I),
+    'qv_mm8': ([_P] * 5 + [_I] * 3 + [_P], _I),
+    'qv_cache8_pack': ([_P] * 6 + [_I] * 3 + [_P], _I),
+    'qv_cache8_unpack': ([_P] * 6 + [_I] * 2 + [_P], _I),
     'qv_attention_noalloc': ([_P] * 8 + [_I, _I, _F, _P], _I),
 }
 
@@ -94,6 +99,24 @@ def load_library(path=None):
 
 class NativeError(RuntimeError):
     """A library call returned -1; the message is ``qv_error()``."""
+
+
+# Host-side checks of the 8-bit calls, which take their sizes from the tensors: a wrong shape, element
+# size, layout or device is refused here, before an address reaches a kernel.
+def need_tensor(t, itemsize, shape, name, device):
+    if t.element_size() != itemsize or t.shape != shape or not t.is_contiguous() or not t.is_cuda or t.device != device:
+        raise ValueError(f'{name} must be a contiguous CUDA tensor of shape {list(shape)} with {itemsize}-byte elements '
+                         f'on {device}')
+
+
+def need_cache8(key_codes, key_scales, value_codes, value_scales, end, device):
+    blocks = key_codes.shape[0]
+    need_tensor(key_codes, 1, (blocks, 4, 64, 256), 'key_codes', device)
+    need_tensor(value_codes, 1, (blocks, 4, 64, 256), 'value_codes', device)
+    need_tensor(key_scales, 4, (blocks, 4), 'key_scales', device)
+    need_tensor(value_scales, 4, (blocks, 4), 'value_scales', device)
+    if end > 64 * blocks:
+        raise ValueError(f'the cache holds {blocks} blocks of 64 rows, not {end} rows')
 
 
 class HotPath:
@@ -244,6 +267,77 @@ class HotPath:
                                              p(conv), p(decay), p(bias), p(norm), tokens, key_heads, value_heads,
                                              dim, epsilon, p(workspace), workspace.numel() * workspace.element_size(),
                                              self._stream()))
+
+    # -- 8-bit serving ------------------------------------------------------
+    def _call(self, device, function, *args):
+        """function(*args, stream) with the tensors' device current, on torch's current stream of it."""
+        import torch
+        stream = torch.cuda.current_stream(device).cuda_stream
+        if torch.cuda.current_device() == device.index:
+            code = function(*args, stream)
+        else:
+            with torch.cuda.device(device):
+                code = function(*args, stream)
+        self.check(code)
+
+    def norm8(self, codes, scales, x, weights, residual=None, residual_out=None, normed=None, epsilon=1e-6):
+        """qv_norm8: e4m3 codes [tokens][width] and scales [ceil(width/128)][tokens] of the RMSNorm of
+        x (+ residual); residual_out and normed, where given, receive the sum and the norm in fp32."""
+        tokens, width = x.shape
+        dev = x.device
+        need_tensor(x, 4, (tokens, width), 'x', dev)
+        need_tensor(codes, 1, (tokens, width), 'codes', dev)
+        need_tensor(scales, 4, (-(-width // 128), tokens), 'scales', dev)
+        need_tensor(weights, 4, (width,), 'weights', dev)
+        for name, t in (('residual', residual), ('residual_out', residual_out), ('normed', normed)):
+            if t is not None:
+                need_tensor(t, 4, (tokens, width), name, dev)
+        self._call(dev, self.lib.qv_norm8, codes.data_ptr(), scales.data_ptr(),
+                   None if residual_out is None else residual_out.data_ptr(),
+                   None if normed is None else normed.data_ptr(), x.data_ptr(),
+                   None if residual is None else residual.data_ptr(), weights.data_ptr(), tokens, width, epsilon)
+
+    def quantize8(self, codes, scales, x):
+        """qv_quantize8: e4m3 codes and scales of x itself."""
+        tokens, width = x.shape
+        dev = x.device
+        need_tensor(x, 4, (tokens, width), 'x', dev)
+        need_tensor(codes, 1, (tokens, width), 'codes', dev)
+        need_tensor(scales, 4, (-(-width // 128), tokens), 'scales', dev)
+        self._call(dev, self.lib.qv_quantize8, codes.data_ptr(), scales.data_ptr(), x.data_ptr(), tokens, width)
+
+    def mm8(self, out, weights, weight_scales, codes, scales):
+        """qv_mm8: out [tokens][rows] = codes x weights^T, both e4m3 with a scale for every block of 128."""
+        tokens, width = codes.shape
+        rows, blocks, dev = weights.shape[0], -(-width // 128), codes.device
+        need_tensor(codes, 1, (tokens, width), 'codes', dev)
+        need_tensor(scales, 4, (blocks, tokens), 'scales', dev)
+        need_tensor(weights, 1, (rows, width), 'weights', dev)
+        need_tensor(weight_scales, 4, (-(-rows // 128), blocks), 'weight_scales', dev)
+        need_tensor(out, 4, (tokens, rows), 'out', dev)
+        self._call(dev, self.lib.qv_mm8, out.data_ptr(), weights.data_ptr(), weight_scales.data_ptr(), codes.data_ptr(),
+                   scales.data_ptr(), tokens, width, rows)
+
+    def cache8_pack(self, key_codes, key_scales, value_codes, value_scales, key_rows, value_rows, begin, end):
+        """qv_cache8_pack: positions [begin, end) of fp16 rows (position r at row r % rows) to int8 codes."""
+        ring, dev = key_rows.shape[0], key_rows.device
+        need_cache8(key_codes, key_scales, value_codes, value_scales, end, dev)
+        need_tensor(key_rows, 2, (ring, 4, 256), 'key_rows', dev)
+        need_tensor(value_rows, 2, (ring, 4, 256), 'value_rows', dev)
+        self._call(dev, self.lib.qv_cache8_pack, key_codes.data_ptr(), key_scales.data_ptr(), value_codes.data_ptr(),
+                   value_scales.data_ptr(), key_rows.data_ptr(), value_rows.data_ptr(), begin, end, ring)
+
+    def cache8_unpack(self, key_rows, value_rows, key_codes, key_scales, value_codes, value_scales, begin, end, origin=0):
+        """qv_cache8_unpack: positions [begin, end) as fp16 rows, position r at row r - origin."""
+        rows, dev = key_rows.shape[0], key_rows.device
+        need_cache8(key_codes, key_scales, value_codes, value_scales, end, dev)
+        need_tensor(key_rows, 2, (rows, 4, 256), 'key_rows', dev)
+        need_tensor(value_rows, 2, (rows, 4, 256), 'value_rows', dev)
+        if not 0 <= begin - origin <= end - origin <= rows:
+            raise ValueError(f'positions [{begin}, {end}) do not fit {rows} rows from position {origin}')
+        skip = (begin - origin) * 2048
+        self._call(dev, self.lib.qv_cache8_unpack, key_rows.data_ptr() + skip, value_rows.data_ptr() + skip,
+                   key_codes.data_ptr(), key_scales.data_ptr(), value_codes.data_ptr(), value_scales.data_ptr(), begin, end)
 
     def status(self):
         """Synchronise and return the kernel status word (0 = no timeout)."""
