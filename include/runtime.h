@@ -359,6 +359,32 @@ int qv_cache8_unpack(void *key_rows, void *value_rows, const void *key_codes,
                      const float *key_scales, const void *value_codes,
                      const float *value_scales, int begin, int end, void *stream);
 
+/* The attention layer of qv_attention for 1..10 new tokens over a cache held
+ * in 8 bits: positions [0, packed) are the blocks that qv_cache8_pack wrote
+ * (packed a multiple of 64, packed <= position), positions from `packed` on
+ * are fp16 rows of key_tail / value_tail [tail_rows][4][256], position r at
+ * row r % tail_rows, with position + batch - packed <= tail_rows.  The new
+ * tokens' keys (normalised, rotated) and values are appended to the tail; no
+ * other row and no packed block is written.  Once position - packed >= 64 the
+ * oldest rows may be packed (qv_cache8_pack with ring_rows = tail_rows, a
+ * multiple of 64): rows before `position` are never written again, so verify
+ * and roll-back need no more than they do with the fp16 cache.
+ * Buffers and arithmetic are qv_attention's otherwise; a new token whose
+ * values are not finite reaches the outputs of the tokens that see it, and no
+ * others.  packed == 0: the code and scale buffers may be null.
+ * `workspace`: qv_attention8_workspace(batch, position) bytes (0 = invalid
+ * arguments), 256-byte aligned, zero-filled once before its first use; it
+ * serves one call at a time, so graphs that may run at the same time need one
+ * each. */
+size_t qv_attention8_workspace(int batch, int position);
+int qv_attention8(float *out, const void *key_codes, const float *key_scales,
+                  const void *value_codes, const float *value_scales, int packed,
+                  void *key_tail, void *value_tail, int tail_rows,
+                  const float *q_gate, const float *key, const float *value,
+                  const float *q_norm, const float *k_norm,
+                  int batch, int position, float epsilon,
+                  void *workspace, size_t workspace_bytes, void *stream);
+
 /* Synchronise the current device and return (then clear) the status word
  * that kernels set when a bounded internal wait gives up: 0 = none. */
 int qv_status(void);

@@ -6,6 +6,8 @@ the values that their codes stand for.
 """
 import numpy as np
 
+from .hotpath import prepare_rows, sigmoid
+
 BLOCK, COLS = 64, 128
 
 
@@ -68,3 +70,24 @@ def unpack(codes, scales):
     """The values of the codes, float64 rows [64 n][4][256]."""
     v = codes.astype(np.float64) * scales.astype(np.float64)[:, :, None, None]
     return v.transpose(0, 2, 1, 3).reshape(-1, 4, 256)
+
+
+def attention(key_rows, value_rows, q_gate, q_norm, position, epsilon=1e-6):
+    """(out [T][24][256], the sum of p |v| times the gate, the largest sum |q k| / 16 of any score), float64:
+    queries at position .. position + T - 1 over the rows [0, position + t] of float64 K/V [n][4][256]."""
+    T = q_gate.shape[0]
+    q = prepare_rows(q_gate[..., :256], q_norm, position + np.arange(T)[:, None], epsilon)
+    gate = sigmoid(q_gate[..., 256:])
+    out, size, top = np.zeros((T, 24, 256)), np.zeros((T, 24, 256)), 0.0
+    for h in range(24):
+        k, v = key_rows[:, h // 6], value_rows[:, h // 6]
+        for t in range(T):
+            n = position + t + 1
+            s = k[:n] @ q[t, h] / 16
+            with np.errstate(invalid='ignore'):
+                top = max(top, float(np.nanmax(np.abs(k[:n]) @ np.abs(q[t, h]))) / 16)
+                p = np.exp(s - s.max())
+                p /= p.sum()
+                out[t, h] = p @ v[:n] * gate[t, h]
+                size[t, h] = p @ np.abs(v[:n]) * gate[t, h]
+    return out, size, top

@@ -20,8 +20,8 @@ CSRC = ROOT / 'redshift_b200' / 'csrc'
 BUILD = ROOT / 'build'
 LIBRARY = BUILD / 'libqvelox.so'
 SOURCES = ['status.cu', 'attention.cu', 'delta.cu', 'gdn_chunk.cu', 'delta_prefill.cu', 'prefill.cu', 'projection.cu', 'copy.cu',
-           'quant8.cu', 'mm8.cu',           'runtime.cu', 'noalloc.cu']
-HEADERS = ['common.cuh', 'hotpath.h']
+           'attention8.cu', 'quant8.cu', 'mm8.cu',           'runtime.cu', 'noalloc.cu']
+HEADERS = ['common.cuh', 'attention_core.cuh', 'hotpath.h']
 
 NVCC_FLAGS = [
     '-gencode', 'arch=compute_100a,code=sm_100a',

@@ -85,6 +85,13 @@ void cache8_pack(int8_t *kc, float *ks, int8_t *vc, float *vs, const __half *k, 
                  int ring, cudaStream_t st);
 void cache8_unpack(__half *k, __half *v, const int8_t *kc, const float *ks, const int8_t *vc, const float *vs, int begin,
                    int end, cudaStream_t st);
+// Decode / verify attention (attention8.cu) over packed blocks [0, packed / 64)
+// and the fp16 ring k_tail / v_tail, where position r >= packed is row r % ring.
+size_t attention8_workspace_bytes(int kv_rows);
+void attention8_run(float *out, const int8_t *kc, const float *ks, const int8_t *vc, const float *vs, int packed,
+                    __half *k_tail, __half *v_tail, int ring, const float *q_gate, const float *key, const float *value,
+                    const float *qn, const float *kn, int T, int position, float eps, void *ws, size_t ws_bytes,
+                    cudaStream_t st);
 // e4m3 codes [tokens][width] with scales [ceil(width/128)][tokens] of x, or with
 // weights of the RMSNorm of x (+ residual); sum_out, normed and residual may be null.
 void norm8(uint8_t *codes, float *scales, float *sum_out, float *normed, const float *x, const float *residual,

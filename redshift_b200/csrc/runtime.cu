@@ -574,6 +574,35 @@ int qv_cache8_unpack(void *key_rows, void *value_rows, const void *key_codes, co
     });
 }
 
+size_t qv_attention8_workspace(int batch, int position) {
+    if (batch < 1 || batch > qv::attention_max_shard_batch() || position < 0 || position > kMaxContext - batch) return 0;
+    return qv::attention8_workspace_bytes(position + batch);
+}
+
+int qv_attention8(float *out, const void *key_codes, const float *key_scales, const void *value_codes,
+                  const float *value_scales, int packed, void *key_tail, void *value_tail, int tail_rows,
+                  const float *q_gate, const float *key, const float *value, const float *q_norm, const float *k_norm,
+                  int batch, int position, float epsilon, void *workspace, size_t workspace_bytes, void *stream) {
+    return guarded([&] {
+        require(batch >= 1 && batch <= qv::attention_max_shard_batch(), "batch must be between 1 and 10");
+        check_epsilon(epsilon);
+        require(position >= 0 && position <= kMaxContext - batch, "attention context exceeds 139264");
+        require(packed >= 0 && packed <= position && packed % qv::CACHE8_BLOCK == 0,
+                "packed rows must be whole blocks of 64 before the position");
+        require(tail_rows > 0 && position + batch - packed <= tail_rows, "the tail does not hold the rows behind the packed ones");
+        require(out && key_tail && value_tail && q_gate && key && value && q_norm && k_norm && workspace &&
+                (packed == 0 || (key_codes && key_scales && value_codes && value_scales)), "null attention buffer");
+        require(aligned16(key_codes) && aligned16(value_codes) && aligned16(key_tail) && aligned16(value_tail) &&
+                aligned16(q_gate) && aligned16(key) && aligned16(value) && aligned16(q_norm) && aligned16(k_norm),
+                "attention buffers must be 16-byte aligned");
+        require((reinterpret_cast<uintptr_t>(workspace) & 255) == 0, "the workspace must be 256-byte aligned");
+        qv::attention8_run(out, static_cast<const int8_t *>(key_codes), key_scales, static_cast<const int8_t *>(value_codes),
+                           value_scales, packed, static_cast<__half *>(key_tail), static_cast<__half *>(value_tail),
+                           tail_rows, q_gate, key, value, q_norm, k_norm, batch, position, epsilon, workspace,
+                           workspace_bytes, as_stream(stream));
+    });
+}
+
 int qv_norm8(void *codes, float *scales, float *residual_out, float *normed, const float *x, const float *residual,
              const float *weights, int tokens, int width, float epsilon, void *stream) {
     return guarded([&] {

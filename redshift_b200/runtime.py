@@ -65,6 +65,8 @@ ADDITIVE_SIGNATURES = {
     'qv_norm8': ([_P] * 7 + [_I, _I, _F, _P], _I),
     'qv_quantize8': ([_P] * 3 + [_I, _I, _P], _I),
     'qv_mm8': ([_P] * 5 + [_I] * 3 + [_P], _I),
+    'qv_attention8_workspace': ([_I, _I], _S),
+    'qv_attention8': ([_P] * 5 + [_I, _P, _P, _I] + [_P] * 5 + [_I, _I, _F, _P, _S, _P], _I),
     'qv_cache8_pack': ([_P] * 6 + [_I] * 3 + [_P], _I),
     'qv_cache8_unpack': ([_P] * 6 + [_I] * 2 + [_P], _I),
     'qv_attention_noalloc': ([_P] * 8 + [_I, _I, _F, _P], _I),
@@ -130,6 +132,7 @@ class HotPath:
     def __init__(self, library=None):
         self.lib = load_library(library)
         self._workspace = None
+        self._workspaces8 = {}
 
     # -- helpers ---------------------------------------------------------
     def check(self, code):
@@ -317,6 +320,46 @@ class HotPath:
         need_tensor(out, 4, (tokens, rows), 'out', dev)
         self._call(dev, self.lib.qv_mm8, out.data_ptr(), weights.data_ptr(), weight_scales.data_ptr(), codes.data_ptr(),
                    scales.data_ptr(), tokens, width, rows)
+
+    def attention8_workspace(self, device):
+        """A new workspace for attention8 at any batch and position: the barrier words in its first 256 bytes
+        are zero.  One serves one call at a time; a captured graph keeps one of its own."""
+        import torch
+        # the split partials of the longest context, which no shorter one exceeds
+        need = max(self.lib.qv_attention8_workspace(1, 139263), self.lib.qv_attention8_workspace(1, 64 * 37 - 1))
+        ws = torch.empty(need, dtype=torch.uint8, device=device)
+        ws[:256].zero_()
+        return ws
+
+    def attention8(self, out, key_codes, key_scales, value_codes, value_scales, packed, key_tail, value_tail, q_gate,
+                   key, value, q_norm, k_norm, batch, position, epsilon=1e-6, workspace=None):
+        """qv_attention8: one attention layer for 1..10 new tokens over the 8-bit cache's first `packed`
+        positions and the fp16 tail.  Without `workspace`, one that is kept for the current stream is used;
+        under graph capture it has to be given (attention8_workspace), since the graph goes on using it."""
+        import torch
+        dev, tail = out.device, key_tail.shape[0]
+        need_tensor(out, 4, (batch, 24, 256), 'out', dev)
+        need_tensor(q_gate, 4, (batch, 24, 512), 'q_gate', dev)
+        need_tensor(key, 4, (batch, 4, 256), 'key', dev)
+        need_tensor(value, 4, (batch, 4, 256), 'value', dev)
+        need_tensor(q_norm, 4, (256,), 'q_norm', dev)
+        need_tensor(k_norm, 4, (256,), 'k_norm', dev)
+        need_tensor(key_tail, 2, (tail, 4, 256), 'key_tail', dev)
+        need_tensor(value_tail, 2, (tail, 4, 256), 'value_tail', dev)
+        need_cache8(key_codes, key_scales, value_codes, value_scales, packed, dev)
+        if workspace is None:
+            if torch.cuda.is_current_stream_capturing():
+                raise ValueError('attention8 under graph capture needs a workspace of its own (attention8_workspace)')
+            which = (dev.index, torch.cuda.current_stream(dev).cuda_stream)
+            workspace = self._workspaces8.get(which)
+            if workspace is None:
+                workspace = self._workspaces8[which] = self.attention8_workspace(dev)
+        else:
+            need_tensor(workspace, 1, workspace.shape, 'workspace', dev)
+        self._call(dev, self.lib.qv_attention8, out.data_ptr(), key_codes.data_ptr(), key_scales.data_ptr(),
+                   value_codes.data_ptr(), value_scales.data_ptr(), packed, key_tail.data_ptr(), value_tail.data_ptr(), tail,
+                   q_gate.data_ptr(), key.data_ptr(), value.data_ptr(), q_norm.data_ptr(), k_norm.data_ptr(),
+                   batch, position, epsilon, workspace.data_ptr(), workspace.numel())
 
     def cache8_pack(self, key_codes, key_scales, value_codes, value_scales, key_rows, value_rows, begin, end):
         """qv_cache8_pack: positions [begin, end) of fp16 rows (position r at row r % rows) to int8 codes."""
