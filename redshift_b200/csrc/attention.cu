@@ -341,7 +341,7 @@ fa_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
     if (o_ready) {
         tc_fence_after();
         static_assert(EPILOGUE_BYTES <= STAGES3 * L::SM_KV_STAGE, "O staging exceeds the K/V ring");
-        store_partials<0>(p, kv_head, tmem, smem + L::SM_KV);
+        store_partials(p, kv_head, tmem, smem + L::SM_KV);
     }
     tc_fence_before();
     __syncthreads();

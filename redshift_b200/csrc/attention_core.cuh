@@ -572,13 +572,11 @@ __device__ __forceinline__ uint32_t append_rows(const FaParams &p, int kv_head, 
 
 // Epilogue of a decode CTA (its first 8 warps), once O is complete and the K/V
 // ring idle.  Warps w and w+4 share TMEM lane quarter w%4 (O_hi of row
-// 16(w%4)+i in lane i, O_lo in lane 16+i, which is 2^LO_SHIFT times its value)
-// and take O columns [0,128) (warps 4-7) and [128,256) (warps 0-3): each lane
+// 16(w%4)+i in lane i, O_lo in lane 16+i) and take O columns [0,128) (warps 4-7) and [128,256) (warps 0-3): each lane
 // puts its lane's columns into a padded staging row, then the warp stores each
 // of its rows, the sum of its hi and lo staging rows, as 512-byte pieces of
 // this split's unnormalised partial.  `ring`: EPILOGUE_BYTES of shared memory.
 constexpr int EPILOGUE_BYTES = 8 * 32 * (128 * 4 + 16);
-template <int LO_SHIFT>
 __device__ __forceinline__ void store_partials(const FaParams &p, int kv_head, uint32_t tmem, uint8_t *ring) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, wq = warp & 3;
     const uint32_t t_lane = tmem + ((uint32_t)(wq * 32) << 16);
@@ -613,12 +611,7 @@ __device__ __forceinline__ void store_partials(const FaParams &p, int kv_head, u
         const int rr = row0 + i;
         float4 v = *reinterpret_cast<const float4 *>(stage + i * RS + col * 4);
         const float4 w = *reinterpret_cast<const float4 *>(stage + (i + 16) * RS + col * 4);
-        if (LO_SHIFT == 0) {
-            v.x += w.x; v.y += w.y; v.z += w.z; v.w += w.w;
-        } else {
-            constexpr float f = 1.f / (1 << LO_SHIFT);
-            v.x = fmaf(w.x, f, v.x); v.y = fmaf(w.y, f, v.y); v.z = fmaf(w.z, f, v.z); v.w = fmaf(w.w, f, v.w);
-        }
+        v.x += w.x; v.y += w.y; v.z += w.z; v.w += w.w;
         float *dst = p.part_o + (((size_t)kv_head * DECODE_ROWS + rr) * p.splits + blockIdx.x) * HD;
         *reinterpret_cast<float4 *>(dst + chalf * 128 + col) = v;
     }
