@@ -12,15 +12,17 @@
 //
 // Bound by the cache's bytes, 2 KB a position.  What keeps the tensor cores fed
 // at twice the fp16 cache's tile rate:
-//  * a block of one head is 16 KB in a row: one bulk copy each, into a ring of
-//    six (96 KB in flight per SM);
-//  * four converter warps write the codes as exact fp16 integers into the MMA's
-//    swizzled operand images, without bank conflicts on either side;
-//  * the softmax reads its scores as 16-lane fragments, which puts the hi and lo
-//    halves of a score into the same thread, and writes the probabilities back to
-//    TMEM over them, where the PV MMA reads its A operand;
-//  * the MMA warp issues as one (mma_f16_ts_by), which keeps it fast beside warps
-//    that use every issue slot.
+//  * eight converter warps (four for K, four for V) write the codes as exact fp16
+//    integers into the MMA's swizzled operand images.  A warp owns 16 rows of
+//    every tile, 4 KB in a row, and brings them into its own ring of three slots
+//    with one bulk copy each (96 KB in flight per SM, no barrier between warps);
+//  * the eight warps that prepared the queries are the softmax, two for each
+//    quarter of TMEM's lanes, 32 columns each.  They read their scores as 16-lane
+//    fragments, which puts the hi and lo halves of a score into the same thread,
+//    and write the probabilities back to TMEM over them, where the PV MMA reads
+//    its A operand;
+//  * a warp of its own issues the MMAs, as one (mma_f16_ts_by), which keeps the
+//    issue fast beside warps that use every slot.
 // The rest is the fp16 kernel's: queries in TMEM as fp16 hi + lo rows, a lazily
 // moved maximum, probabilities as fp16 hi + lo rows, one CTA per (split, K/V
 // head), the splits combined in the tail.
@@ -42,17 +44,20 @@ namespace qv {
 namespace {
 
 constexpr int IMAGES = 2;        // fp16 tile images (K and V each)
-constexpr int RAW_SLOTS = 6;     // tiles of codes in flight
+constexpr int RAW_SLOTS = 3;     // code tiles in flight (K and V each)
+constexpr int WARP_ROWS = 16, WARP_BYTES = WARP_ROWS * HD;        // a converter warp's part of a code tile
+constexpr int SOFT_WARPS = 8, CONV_WARPS = 4, THREADS8 = 32 * (SOFT_WARPS + 2 * CONV_WARPS + 1);
 constexpr int CODES_TILE = BN * HD;                               // codes of one (block, head)
 constexpr float P_BIAS = 6.f;    // log2 units above the running maximum
 struct A8Layout {
     static constexpr int SM_KV = 0;                               // images: (K, V) of two tiles
     static constexpr int SM_KV_STAGE = 2 * TILE_BYTES;
-    static constexpr int SM_RAW = SM_KV + IMAGES * SM_KV_STAGE;   // ring of code tiles, K and V in turn
-    static constexpr int SM_QSTAGE = SM_RAW + 4 * CODES_TILE;     // slots 4 and 5 until the queries are in TMEM
-    static constexpr int SM_BAR = SM_RAW + RAW_SLOTS * CODES_TILE;
-    static constexpr int SM_ROPE = SM_BAR + 256;                  // (cos, sin) [T][32]
+    static constexpr int SM_RAW = SM_KV + IMAGES * SM_KV_STAGE;   // code tiles [slot][K, V]
+    static constexpr int SM_QSTAGE = SM_RAW + 4 * CODES_TILE;     // slot 2 until the queries are in TMEM
+    static constexpr int SM_BAR = SM_RAW + RAW_SLOTS * 2 * CODES_TILE;
+    static constexpr int SM_ROPE = SM_BAR + 512;                  // (cos, sin) [T][32]; then the maxima [2][2][64] and sums [64]
     static constexpr int SMEM_BYTES = SM_ROPE + MAX_DECODE_T * 32 * 8;
+    static_assert(5 * DECODE_ROWS * 4 <= MAX_DECODE_T * 32 * 8);
 };
 static_assert(A8Layout::SMEM_BYTES <= 227 * 1024, "attention kernel exceeds the shared memory of a CTA");
 static_assert(EPILOGUE_BYTES <= A8Layout::SM_BAR, "O staging exceeds the images and the ring");
@@ -71,21 +76,20 @@ __device__ __forceinline__ uint32_t fp16_codes(uint32_t biased, uint32_t select)
     const uint32_t w = __byte_perm(biased, 0x64646464u, select);
     return half2_bits(__hsub2(*reinterpret_cast<const __half2 *>(&w), __half2half2(__ushort_as_half(0x6480))));
 }
-__global__ void __launch_bounds__(384, 1) attention8_kernel(const FaParams p, const Cache8View c) {
+__global__ void __launch_bounds__(THREADS8, 1) attention8_kernel(const FaParams p, const Cache8View c) {
     using L = A8Layout;
-    constexpr int SOFT_WARPS = 4, CONV_WARPS = 4;
     extern __shared__ __align__(1024) uint8_t smem[];
     if (smem_addr(smem) & 1023) {           // 128B-swizzle atoms need a 1024-byte aligned base
         if (threadIdx.x == 0) raise_status(STATUS_BAD_ARGUMENT);
         return;
     }
-    uint64_t *raw_full = reinterpret_cast<uint64_t *>(smem + L::SM_BAR), *raw_empty = raw_full + RAW_SLOTS;
-    uint64_t *k_full = raw_empty + RAW_SLOTS, *v_full = k_full + 2, *k_empty = k_full + 4, *v_empty = k_full + 6,
+    uint64_t *raw_full = reinterpret_cast<uint64_t *>(smem + L::SM_BAR);         // [8 warps][RAW_SLOTS]
+    uint64_t *k_full = raw_full + 8 * RAW_SLOTS, *v_full = k_full + 2, *k_empty = k_full + 4, *v_empty = k_full + 6,
              *s_full = k_full + 8, *p_full = k_full + 10, *p_free = k_full + 12, *mma_done = k_full + 14,
-             *q_ready = k_full + 15, *app_done = k_full + 16, *cbar = k_full + 17;      // 30 barriers
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + L::SM_BAR + 240);
-    volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + L::SM_BAR + 244);
-    uint32_t *bad_values = reinterpret_cast<uint32_t *>(smem + L::SM_BAR + 248);
+             *q_ready = k_full + 15, *app_done = k_full + 16, *cbar = k_full + 17, *q_loaded = k_full + 18, *exchanged = k_full + 19;   // 51 in all
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + L::SM_BAR + 416);
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + L::SM_BAR + 420);
+    uint32_t *bad_values = reinterpret_cast<uint32_t *>(smem + L::SM_BAR + 424);
     float2 *rope = reinterpret_cast<float2 *>(smem + L::SM_ROPE);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -102,7 +106,7 @@ __global__ void __launch_bounds__(384, 1) attention8_kernel(const FaParams p, co
         prefetch_l2(p.q_gate + ((size_t)(rr / GROUP) * NQ + kv_head * GROUP + rr % GROUP) * 2 * HD + (i & 7) * 32);
     }
     if (threadIdx.x == 0) {
-        for (int i = 0; i < RAW_SLOTS; ++i) { mbar_init(raw_full + i, 1); mbar_init(raw_empty + i, CONV_WARPS); }
+        for (int i = 0; i < 8 * RAW_SLOTS; ++i) mbar_init(raw_full + i, 1);
         for (int i = 0; i < 2; ++i) {
             mbar_init(k_full + i, CONV_WARPS); mbar_init(v_full + i, CONV_WARPS);
             mbar_init(k_empty + i, 1); mbar_init(v_empty + i, 1);
@@ -112,6 +116,8 @@ __global__ void __launch_bounds__(384, 1) attention8_kernel(const FaParams p, co
         mbar_init(q_ready, 8);
         mbar_init(cbar, 1);
         mbar_init(app_done, 64);
+        mbar_init(q_loaded, 1);
+        for (int i = 0; i < 8; ++i) mbar_init(exchanged + i, 2);
         *abort_flag = 0;
         *bad_values = 0;
         fence_barrier_init();
@@ -124,38 +130,42 @@ __global__ void __launch_bounds__(384, 1) attention8_kernel(const FaParams p, co
     grid_dependency_wait();
     if (threadIdx.x == 0) launch_dependents();
 
-    // Tiles of codes among this CTA's (the first ones), as halves: tile j's K is 2 j, its V 2 j + 1.
-    const int code_tiles = max(0, min(ntiles, c.blocks - tile0));
-    auto issue_half = [&](int h) {
-        const int8_t *src = (h & 1 ? c.vc : c.kc) + ((size_t)(tile0 + (h >> 1)) * NKV + kv_head) * CODES_TILE;
-        uint64_t *bar = raw_full + h % RAW_SLOTS;
-        mbar_expect_tx(bar, CODES_TILE);
-        bulk_load(smem + L::SM_RAW + h % RAW_SLOTS * CODES_TILE, src, CODES_TILE, bar);
-    };
+    const int code_tiles = max(0, min(ntiles, c.blocks - tile0));       // tiles of codes, the first of this CTA's
 
-    if (warp >= 8) {
-        // ------------------------------------------------ converters
+    if (warp >= SOFT_WARPS && warp < SOFT_WARPS + 2 * CONV_WARPS) {
+        // ------------------------------------------------ converters (warps 8-11: K, 12-15: V)
         // A lane takes 16 codes (16 dims of a row) at a time: 16 bytes of the
         // code tile, two 16-byte chunks of a 64-dim box of the image.  Eight
-        // lanes are four neighbouring pieces of an even row in box w and four of
-        // the odd row after it in box w ^ 1: their loads cover the two halves of
-        // 128 bytes and their stores, swizzled by the row, even and odd chunks.
-        const int w = warp - 8, q = lane & 3, row0 = lane >> 2, box = w ^ (row0 & 1), piece = 4 * box + q;
-        const uint32_t from = row0 * HD + piece * 16;
+        // lanes are four neighbouring pieces of an even row and four, in the
+        // box's neighbour, of the odd row after it: their loads cover the two
+        // halves of 128 bytes and their stores, swizzled by the row, even and
+        // odd chunks.
+        const int part = (warp - SOFT_WARPS) >> 2, w = warp & 3, q = lane & 3, odd = lane >> 2 & 1;
+        const int box = (lane >> 3) ^ odd, piece = 4 * box + q, row0 = WARP_ROWS * w + odd;
         const uint32_t image = box * (BN * 128) + row0 * 128;
-        const uint32_t at0 = image + (((2 * q) ^ row0) << 4), at1 = image + (((2 * q + 1) ^ row0) << 4);
-        auto convert = [&](uint8_t *dst, int h) {
+        const int8_t *codes = (part ? c.vc : c.kc) + ((size_t)tile0 * NKV + kv_head) * CODES_TILE + w * WARP_BYTES;
+        uint8_t *ring = smem + L::SM_RAW + part * CODES_TILE + w * WARP_BYTES;
+        uint64_t *landed = raw_full + (warp - SOFT_WARPS) * RAW_SLOTS;
+        int issued = 0;
+        auto fetch = [&](int j) {                               // one lane: tile j's rows of this warp
+            const int slot = j % RAW_SLOTS;
+            mbar_expect_tx(landed + slot, WARP_BYTES);
+            bulk_load(ring + slot * 2 * CODES_TILE, codes + (size_t)j * (NKV * CODES_TILE), WARP_BYTES, landed + slot);
+        };
+        auto convert = [&](uint8_t *dst, int j) {
             uint4 x[8];
-            const uint8_t *src = smem + L::SM_RAW + h % RAW_SLOTS * CODES_TILE + from;
+            const uint8_t *src = ring + j % RAW_SLOTS * 2 * CODES_TILE + odd * HD + piece * 16;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = *reinterpret_cast<const uint4 *>(src + i * 8 * HD);
+            for (int i = 0; i < 8; ++i) x[i] = *reinterpret_cast<const uint4 *>(src + i * 2 * HD);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const uint32_t w0 = x[i].x ^ 0x80808080u, w1 = x[i].y ^ 0x80808080u;
                 const uint32_t w2 = x[i].z ^ 0x80808080u, w3 = x[i].w ^ 0x80808080u;
-                *reinterpret_cast<uint4 *>(dst + at0 + i * 1024) =
+                uint8_t *d = dst + image + i * 256;
+                const int swizzle = (2 * i + odd) & 7;
+                *reinterpret_cast<uint4 *>(d + (((2 * q) ^ swizzle) << 4)) =
                     make_uint4(fp16_codes(w0, 0x4140), fp16_codes(w0, 0x4342), fp16_codes(w1, 0x4140), fp16_codes(w1, 0x4342));
-                *reinterpret_cast<uint4 *>(dst + at1 + i * 1024) =
+                *reinterpret_cast<uint4 *>(d + (((2 * q + 1) ^ swizzle) << 4)) =
                     make_uint4(fp16_codes(w2, 0x4140), fp16_codes(w2, 0x4342), fp16_codes(w3, 0x4140), fp16_codes(w3, 0x4342));
             }
         };
@@ -164,14 +174,16 @@ __global__ void __launch_bounds__(384, 1) attention8_kernel(const FaParams p, co
             const int pos0 = (tile0 + j) * BN + row0;
 #pragma unroll 4
             for (int i = 0; i < 8; ++i) {
-                const int pos = pos0 + 8 * i;
+                const int pos = pos0 + 2 * i;
                 uint4 a = make_uint4(0u, 0u, 0u, 0u), b = a;
                 if (pos < p.kv_rows && !(pos >= p.position && (skip >> (pos - p.position) & 1u))) {
                     const uint4 *src = reinterpret_cast<const uint4 *>(rows + ((size_t)(pos % c.ring) * NKV + kv_head) * HD + piece * 16);
                     a = src[0]; b = src[1];
                 }
-                *reinterpret_cast<uint4 *>(dst + at0 + i * 1024) = a;
-                *reinterpret_cast<uint4 *>(dst + at1 + i * 1024) = b;
+                uint8_t *d = dst + image + i * 256;
+                const int swizzle = (2 * i + odd) & 7;
+                *reinterpret_cast<uint4 *>(d + (((2 * q) ^ swizzle) << 4)) = a;
+                *reinterpret_cast<uint4 *>(d + (((2 * q + 1) ^ swizzle) << 4)) = b;
             }
         };
         auto publish = [&](uint64_t *bar) {
@@ -179,63 +191,45 @@ __global__ void __launch_bounds__(384, 1) attention8_kernel(const FaParams p, co
             __syncwarp();
             if (lane == 0) mbar_arrive(bar);
         };
+        uint64_t *full = part ? v_full : k_full, *empty = part ? v_empty : k_empty;
+        const __half *rows = part ? p.vc : p.kc;
+        // The first copies go out once the query rows have arrived (issued before
+        // them they would queue in front), the last slot once it stages no queries.
+        if (code_tiles > 0 && warp_wait(q_loaded, 0, abort_flag)) {
+            issued = min(code_tiles, RAW_SLOTS - 1);
+            if (lane == 0) for (int j = 0; j < issued; ++j) fetch(j);
+            if (issued < code_tiles && warp_wait(q_ready, 0, abort_flag)) {
+                fence_async_shared();            // the staged queries were written and read by plain accesses
+                if (lane == 0) fetch(issued);
+                ++issued;
+            }
+        }
         for (int j = 0; j < ntiles; ++j) {
             const int s = j & 1;
-            const uint32_t before = (uint32_t)((j >> 1) - 1) & 1;
-            uint8_t *kd = smem + L::SM_KV + s * L::SM_KV_STAGE;
+            uint8_t *dst = smem + L::SM_KV + s * L::SM_KV_STAGE + part * TILE_BYTES;
             const bool fresh = appends && (tile0 + j + 1) * BN > p.position;      // the tile holds new rows
-            bool ok = true;
-            for (int part = 0; part < 2 && ok; ++part) {                           // K, then V
-                const int h = 2 * j + part;
-                uint8_t *dst = kd + part * TILE_BYTES;
-                if (j >= 2) ok = warp_wait((part ? v_empty : k_empty) + s, before, abort_flag);
-                if (j < code_tiles) {
-                    ok = ok && warp_wait(raw_full + h % RAW_SLOTS, (uint32_t)(h / RAW_SLOTS) & 1, abort_flag);
-                    if (!ok) break;
-                    convert(dst, h);
-                } else {
-                    ok = ok && (!fresh || warp_wait(app_done, 0, abort_flag));
-                    if (!ok) break;
-                    copy_rows(dst, part ? p.vc : p.kc, j, part && fresh ? *reinterpret_cast<volatile uint32_t *>(bad_values) : 0u);
-                }
-                publish((part ? v_full : k_full) + s);
-                if (j < code_tiles && lane == 0) mbar_arrive(raw_empty + h % RAW_SLOTS);
+            if (j < code_tiles) {
+                if (!warp_wait(landed + j % RAW_SLOTS, (uint32_t)(j / RAW_SLOTS) & 1, abort_flag)) break;
+            } else if (fresh && !warp_wait(app_done, 0, abort_flag)) {
+                break;
             }
-            if (!ok) break;
+            if (j >= 2 && !warp_wait(empty + s, (uint32_t)((j >> 1) - 1) & 1, abort_flag)) break;
+            if (j < code_tiles) convert(dst, j);
+            else copy_rows(dst, rows, j, part && fresh ? *reinterpret_cast<volatile uint32_t *>(bad_values) : 0u);
+            publish(full + s);                   // the slot has been read, too
+            if (issued < code_tiles) {
+                if (lane == 0) fetch(issued);
+                ++issued;
+            }
         }
-        return;                          // the later barriers count the other eight warps
+        // Every issued copy must land before the CTA may exit.
+        const long long t0 = clock64();
+        for (int j = max(0, issued - RAW_SLOTS); j < issued; ++j)
+            while (!mbar_try_wait(landed + j % RAW_SLOTS, (uint32_t)(j / RAW_SLOTS) & 1) && clock64() - t0 < WAIT_LIMIT_CYCLES) {}
+        return;                          // the later barriers count the first eight warps
     }
 
-    // The first tiles' codes are asked for once the query rows have arrived (issued
-    // before them they would queue in front), slots 4 and 5 once they stage no queries.
-    const int early = min(2 * code_tiles, 4);
-    prepare_queries(p, kv_head, rope, smem + L::SM_QSTAGE, tmem, q_ready, [&] { for (int h = 0; h < early; ++h) issue_half(h); });
-    if ((warp == 2 || warp == 3) && appends) {
-        const int ring = c.ring;
-        const uint32_t bad = append_rows<true>(p, kv_head, warp - 2, app_lo, app_hi, rope, [ring](int pos) { return pos % ring; });
-        if (lane == 0 && bad) atomicOr(bad_values, bad);
-        __threadfence_block();
-        mbar_arrive(app_done);
-    }
-
-    if (warp == 0) {
-        // ------------------------------------------------ producer
-        if (lane == 0) {
-            int issued = early;
-            if (2 * code_tiles > early && mbar_wait(q_ready, 0, abort_flag)) {
-                fence_async_shared();            // the staged queries were written and read by plain accesses
-                for (int h = early; h < 2 * code_tiles; ++h) {
-                    if (h >= RAW_SLOTS && !mbar_wait(raw_empty + h % RAW_SLOTS, (uint32_t)(h / RAW_SLOTS - 1) & 1, abort_flag)) break;
-                    issue_half(h);
-                    issued = h + 1;
-                }
-            }
-            // Every issued copy must land before the CTA may exit.
-            const long long t0 = clock64();
-            for (int h = max(0, issued - RAW_SLOTS); h < issued; ++h)
-                while (!mbar_try_wait(raw_full + h % RAW_SLOTS, (uint32_t)(h / RAW_SLOTS) & 1) && clock64() - t0 < WAIT_LIMIT_CYCLES) {}
-        }
-    } else if (warp == 1) {
+    if (warp == SOFT_WARPS + 2 * CONV_WARPS) {
         // ------------------------------------------------ MMA issuer (the whole warp, one elected lane)
         const uint32_t lead = elect_lane(), tm = __shfl_sync(0xffffffffu, tmem, 0);
         const uint32_t idesc_qk = idesc_f16(128, BN, false, false), idesc_pv = idesc_f16(128, HD, false, true);
@@ -273,14 +267,27 @@ __global__ void __launch_bounds__(384, 1) attention8_kernel(const FaParams p, co
         mma_commit_by(lead, mma_done);
         const long long t0 = clock64();
         while (!mbar_try_wait(mma_done, 0) && clock64() - t0 < WAIT_LIMIT_CYCLES) {}
-    } else if (warp >= 4) {
+        return;
+    }
+
+    prepare_queries(p, kv_head, rope, smem + L::SM_QSTAGE, tmem, q_ready, [&] { mbar_arrive(q_loaded); });
+    if ((warp == 2 || warp == 3) && appends) {
+        const int ring = c.ring;
+        const uint32_t bad = append_rows<true>(p, kv_head, warp - 2, app_lo, app_hi, rope, [ring](int pos) { return pos % ring; });
+        if (lane == 0 && bad) atomicOr(bad_values, bad);
+        __threadfence_block();
+        mbar_arrive(app_done);
+    }
+    {
         // ------------------------------------------------ softmax
-        // Lanes 32w + i and 32w + 16 + i of TMEM hold the hi and lo halves of query
-        // row 16w + i.  Thread l of warp w has the rows 16w + l / 4 + 8 u (u = 0,
-        // 1), in each 16 of a tile's 64 columns: 8 n + 2 (l % 4) + e in x[2 n + u].
-        const int wq = warp & 3;
+        // Lanes 32g + i and 32g + 16 + i of TMEM hold the hi and lo halves of query
+        // row 16g + i.  Warp w has the rows of g = w % 4 and the columns 32 (w / 4)
+        // to + 32 of every tile; thread l of it the rows 16g + l / 4 + 8 u (u = 0,
+        // 1) and, of these, the columns 8 n + 2 (l % 4) + e in x[2 n + u].
+        const int wq = warp & 3, part = warp >> 2;
         const uint32_t t_hi = tmem + ((uint32_t)(wq * 32) << 16), t_lo = t_hi + (16u << 16);
         const int r0 = wq * 16 + (lane >> 2), rows = p.T * GROUP;
+        float *maxima = reinterpret_cast<float *>(rope);           // [tile parity][part][64 rows], once the rotary table is used up
         int last[2];                                               // last visible position
         float m_use[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 #pragma unroll
@@ -292,6 +299,7 @@ __global__ void __launch_bounds__(384, 1) attention8_kernel(const FaParams p, co
         };
         float ks, vs;
         scales_of(0, ks, vs);
+        named_barrier(4, 32 * SOFT_WARPS);                         // the append has used the rotary table
         for (int j = 0; j < ntiles; ++j) {
             const int b = j & 1;
             const float to_log2 = SCORE_LOG2 * ks;
@@ -301,18 +309,18 @@ __global__ void __launch_bounds__(384, 1) attention8_kernel(const FaParams p, co
             scales_of(j + 1, ks, vs);
             if (!warp_wait(s_full + b, (j >> 1) & 1, abort_flag)) break;
             tc_fence_after();
-            float2 x[16];
+            float2 x[8];
             {
-                float hi[32], lo[32];
-                tmem_ld_16x256b_x8(t_hi + TM_S + b * BN, hi);
-                tmem_ld_16x256b_x8(t_lo + TM_S + b * BN, lo);
+                float hi[16], lo[16];
+                tmem_ld_16x256b_x4(t_hi + TM_S + b * BN + part * 32, hi);
+                tmem_ld_16x256b_x4(t_lo + TM_S + b * BN + part * 32, lo);
                 tmem_wait_ld();
 #pragma unroll
-                for (int q = 0; q < 16; ++q)
+                for (int q = 0; q < 8; ++q)
                     x[q] = fadd2(make_float2(hi[2 * q], hi[2 * q + 1]), make_float2(lo[2 * q], lo[2 * q + 1]));
             }
             if (j >= code_tiles) {                                 // only fp16 tiles hold positions past a query
-                const int key0 = (tile0 + j) * BN + 2 * (lane & 3);
+                const int key0 = (tile0 + j) * BN + part * 32 + 2 * (lane & 3);
                 uint32_t bad = 0;
                 if (appends && (tile0 + j + 1) * BN > p.position) {
                     if (!warp_wait(app_done, 0, abort_flag)) break;
@@ -327,40 +335,49 @@ __global__ void __launch_bounds__(384, 1) attention8_kernel(const FaParams p, co
                     return key <= last[u] ? v : -INFINITY;
                 };
 #pragma unroll
-                for (int q = 0; q < 16; ++q) {
+                for (int q = 0; q < 8; ++q) {
                     x[q].x = masked(x[q].x, key0 + 8 * (q >> 1), q & 1);
                     x[q].y = masked(x[q].y, key0 + 8 * (q >> 1) + 1, q & 1);
                 }
             }
-            float factor[2];
+            // The row's maximum: this thread's columns, the row's other three
+            // threads, and the warp with the other 32 columns.  Behind the exchange
+            // both warps have read their scores, so P may overwrite them.
+            float m[2], factor[2];
+            float *mine = maxima + (b * 2 + part) * DECODE_ROWS, *other = maxima + (b * 2 + 1 - part) * DECODE_ROWS;
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                m[u] = fmaxf(fmaxf(fmaxf(x[u].x, x[u].y), fmaxf(x[2 + u].x, x[2 + u].y)),
+                             fmaxf(fmaxf(x[4 + u].x, x[4 + u].y), fmaxf(x[6 + u].x, x[6 + u].y)));
+                m[u] = fmaxf(m[u], __shfl_xor_sync(0xffffffffu, m[u], 1));
+                m[u] = fmaxf(m[u], __shfl_xor_sync(0xffffffffu, m[u], 2));
+                if ((lane & 3) == 0) mine[r0 + 8 * u] = m[u];
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(exchanged + 2 * wq + b);
+            if (!warp_wait(exchanged + 2 * wq + b, (j >> 1) & 1, abort_flag)) break;
+            tc_fence_after();
             bool need = false;
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
-                float m0 = fmaxf(x[u].x, x[u].y), m1 = fmaxf(x[2 + u].x, x[2 + u].y);
-#pragma unroll
-                for (int n = 2; n < 8; n += 2) {
-                    m0 = fmaxf(m0, fmaxf(x[2 * n + u].x, x[2 * n + u].y));
-                    m1 = fmaxf(m1, fmaxf(x[2 * n + 2 + u].x, x[2 * n + 2 + u].y));
-                }
-                float m = fmaxf(m0, m1);
-                m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
-                m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-                m = fmaf(m, to_log2, v_log2);                      // log2 units (-inf stays -inf)
+                m[u] = fmaf(fmaxf(m[u], other[r0 + 8 * u]), to_log2, v_log2);     // log2 units (-inf stays -inf)
                 factor[u] = 1.f;
-                if (m > m_use[u] + RESCALE_THRESHOLD) {
-                    factor[u] = exp2_approx(m_use[u] - m);
-                    m_use[u] = m;
+                if (m[u] > m_use[u] + RESCALE_THRESHOLD) {
+                    factor[u] = exp2_approx(m_use[u] - m[u]);
+                    m_use[u] = m[u];
                     l[u] *= factor[u];
                     need = true;
                 }
             }
             if (j > 0 && __any_sync(0xffffffffu, need)) {
-                // O already holds tiles < j: wait for PV(j-1), then rescale its rows.
+                // O already holds tiles < j: wait for PV(j-1), then rescale its rows
+                // (this warp's half of the columns).
                 if (!warp_wait(p_free + ((j - 1) & 1), ((j - 1) >> 1) & 1, abort_flag)) break;
                 tc_fence_after();
 #pragma unroll 1
-                for (int q = 0; q < 2 * HD / 32; ++q) {
-                    const uint32_t at = (q & 1 ? t_lo : t_hi) + TM_O + (q >> 1) * 32;
+                for (int q = 0; q < HD / 32; ++q) {
+                    const uint32_t at = (q & 1 ? t_lo : t_hi) + TM_O + part * (HD / 2) + (q >> 1) * 32;
                     float o[16];
                     uint32_t scaled[16];
                     tmem_ld_16x256b_x4(at, o);
@@ -371,7 +388,7 @@ __global__ void __launch_bounds__(384, 1) attention8_kernel(const FaParams p, co
                 }
                 tmem_wait_st();
             }
-            uint32_t hi[16], lo[16];
+            uint32_t hi[8], lo[8];
             const float2 scale2 = make_float2(to_log2, to_log2), minus = make_float2(-1.f, -1.f);
             float2 shift[2], sum[2];
 #pragma unroll
@@ -381,7 +398,7 @@ __global__ void __launch_bounds__(384, 1) attention8_kernel(const FaParams p, co
                 sum[u] = make_float2(0.f, 0.f);
             }
 #pragma unroll
-            for (int q = 0; q < 16; ++q) {
+            for (int q = 0; q < 8; ++q) {
                 const float2 arg = ffma2(x[q], scale2, shift[q & 1]);
                 const float2 e = make_float2(exp2_approx(arg.x), exp2_approx(arg.y));
                 sum[q & 1] = fadd2(sum[q & 1], e);
@@ -392,24 +409,30 @@ __global__ void __launch_bounds__(384, 1) attention8_kernel(const FaParams p, co
             }
 #pragma unroll
             for (int u = 0; u < 2; ++u) l[u] = fmaf(sum[u].x + sum[u].y, v_inv, l[u]);
-            tmem_st_16x128b_x8(t_hi + TM_S + b * BN, hi);
-            tmem_st_16x128b_x8(t_lo + TM_S + b * BN, lo);
+            tmem_st_16x128b_x4(t_hi + TM_S + b * BN + part * 16, hi);
+            tmem_st_16x128b_x4(t_lo + TM_S + b * BN + part * 16, lo);
             tmem_wait_st();
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(p_full + b);
         }
-        // The rows' running max and sum, for the split combine.
+        // The rows' running max and sum, for the split combine (both warps of a
+        // row moved the same maximum).
+        float *sums = maxima + 4 * DECODE_ROWS;
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
             l[u] += __shfl_xor_sync(0xffffffffu, l[u], 1);
             l[u] += __shfl_xor_sync(0xffffffffu, l[u], 2);
-            if ((lane & 3) == 0 && r0 + 8 * u < rows) {
+            if (part == 1 && (lane & 3) == 0) sums[r0 + 8 * u] = l[u];
+        }
+        named_barrier(8 + wq, 64);
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+            if (part == 0 && (lane & 3) == 0 && r0 + 8 * u < rows) {
                 const size_t slot = ((size_t)kv_head * DECODE_ROWS + r0 + 8 * u) * MAXS + blockIdx.x;
                 p.part_ml[slot * 2] = m_use[u];
-                p.part_ml[slot * 2 + 1] = l[u];
+                p.part_ml[slot * 2 + 1] = l[u] + sums[r0 + 8 * u];
             }
-        }
     }
     // The final PV's commit on p_free marks O complete and every image consumed.
     __syncwarp();
@@ -422,7 +445,7 @@ __global__ void __launch_bounds__(384, 1) attention8_kernel(const FaParams p, co
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    if (warp == 1) tmem_dealloc(tmem, 512);
+    if (warp == 1) tmem_dealloc(tmem, 512);     // the warp that allocated it
     decode_tail(p, kv_head, smem + L::SM_QSTAGE, reinterpret_cast<float *>(smem + L::SM_KV), cbar, abort_flag);
 }
 
@@ -453,7 +476,7 @@ void attention8_run(float *out, const int8_t *kc, const float *ks, const int8_t 
     p.key = key; p.value = value; p.qn = qn; p.kn = kn; p.kc = k_tail; p.vc = v_tail;
     p.append_row0 = position; p.eps = eps;
     const Cache8View c{kc, vc, ks, vs, packed / CACHE8_BLOCK, ring};
-    const cudaError_t e = launch_chained(attention8_kernel, dim3(sp.splits, NKV), dim3(384), A8Layout::SMEM_BYTES, st, p, c);
+    const cudaError_t e = launch_chained(attention8_kernel, dim3(sp.splits, NKV), dim3(THREADS8), A8Layout::SMEM_BYTES, st, p, c);
     if (e != cudaSuccess) throw std::runtime_error(std::string("8-bit attention: ") + cudaGetErrorString(e));
 }
 
