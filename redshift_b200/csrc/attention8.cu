@@ -39,6 +39,7 @@
 #include <algorithm>
 #include <stdexcept>
 #include <string>
+#include <type_traits>
 
 namespace qv {
 namespace {
@@ -48,6 +49,7 @@ constexpr int RAW_SLOTS = 3;     // code tiles in flight (K and V each)
 constexpr int WARP_ROWS = 16, WARP_BYTES = WARP_ROWS * HD;        // a converter warp's part of a code tile
 constexpr int SOFT_WARPS = 8, CONV_WARPS = 4, THREADS8 = 32 * (SOFT_WARPS + 2 * CONV_WARPS + 1);
 constexpr int CODES_TILE = BN * HD;                               // codes of one (block, head)
+constexpr int MAX_TILES8 = 160;  // tiles of a CTA (59 at the longest context on 148 SMs)
 constexpr float P_BIAS = 6.f;    // log2 units above the running maximum
 struct A8Layout {
     static constexpr int SM_KV = 0;                               // images: (K, V) of two tiles
@@ -55,9 +57,9 @@ struct A8Layout {
     static constexpr int SM_RAW = SM_KV + IMAGES * SM_KV_STAGE;   // code tiles [slot][K, V]
     static constexpr int SM_QSTAGE = SM_RAW + 4 * CODES_TILE;     // slot 2 until the queries are in TMEM
     static constexpr int SM_BAR = SM_RAW + RAW_SLOTS * 2 * CODES_TILE;
-    static constexpr int SM_ROPE = SM_BAR + 512;                  // (cos, sin) [T][32]; then the maxima [2][2][64] and sums [64]
+    static constexpr int SM_ROPE = SM_BAR + 512;                  // (cos, sin) [T][32]; then maxima, sums and scales
     static constexpr int SMEM_BYTES = SM_ROPE + MAX_DECODE_T * 32 * 8;
-    static_assert(5 * DECODE_ROWS * 4 <= MAX_DECODE_T * 32 * 8);
+    static_assert((5 * DECODE_ROWS + 2 * MAX_TILES8) * 4 <= MAX_DECODE_T * 32 * 8);
 };
 static_assert(A8Layout::SMEM_BYTES <= 227 * 1024, "attention kernel exceeds the shared memory of a CTA");
 static_assert(EPILOGUE_BYTES <= A8Layout::SM_BAR, "O staging exceeds the images and the ring");
@@ -70,12 +72,25 @@ struct Cache8View {
     int ring;                    // rows of the fp16 ring
 };
 
-// Two fp16 integers of the codes' biased bytes (code + 128): 1024 + byte is the
-// fp16 number 0x6400 | byte, and the difference to 1152 is exact.
-__device__ __forceinline__ uint32_t fp16_codes(uint32_t biased, uint32_t select) {
+// Two fp16 numbers of two codes' biased bytes u = code + 128.  Keys: the
+// subnormal numbers u 2^-24; the bias adds 128 times the sum of the query to
+// every score, which the softmax's argument takes off again at no cost.
+// Values: 1024 + u is the fp16 number 0x6400 | u, and its difference to 1152,
+// the code, is exact (a bias of the values would have to be subtracted from
+// sums a thousand times smaller than it).
+constexpr float KEY_UNIT = 0x1p24f;
+template <bool VALUES> __device__ __forceinline__ uint32_t fp16_pair(uint32_t biased, uint32_t select) {
+    if (!VALUES) return __byte_perm(biased, 0u, select);
     const uint32_t w = __byte_perm(biased, 0x64646464u, select);
     return half2_bits(__hsub2(*reinterpret_cast<const __half2 *>(&w), __half2half2(__ushort_as_half(0x6480))));
 }
+template <bool VALUES> __device__ __forceinline__ uint4 fp16_codes(uint32_t a, uint32_t b) {
+    a ^= 0x80808080u;
+    b ^= 0x80808080u;
+    return make_uint4(fp16_pair<VALUES>(a, 0x4140), fp16_pair<VALUES>(a, 0x4342), fp16_pair<VALUES>(b, 0x4140),
+                      fp16_pair<VALUES>(b, 0x4342));
+}
+
 __global__ void __launch_bounds__(THREADS8, 1) attention8_kernel(const FaParams p, const Cache8View c) {
     using L = A8Layout;
     extern __shared__ __align__(1024) uint8_t smem[];
@@ -152,21 +167,20 @@ __global__ void __launch_bounds__(THREADS8, 1) attention8_kernel(const FaParams 
             mbar_expect_tx(landed + slot, WARP_BYTES);
             bulk_load(ring + slot * 2 * CODES_TILE, codes + (size_t)j * (NKV * CODES_TILE), WARP_BYTES, landed + slot);
         };
-        auto convert = [&](uint8_t *dst, int j) {
+        auto convert = [&](auto values, uint8_t *dst, int j) {
+            constexpr bool V = decltype(values)::value;
             uint4 x[8];
             const uint8_t *src = ring + j % RAW_SLOTS * 2 * CODES_TILE + odd * HD + piece * 16;
 #pragma unroll
             for (int i = 0; i < 8; ++i) x[i] = *reinterpret_cast<const uint4 *>(src + i * 2 * HD);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const uint32_t w0 = x[i].x ^ 0x80808080u, w1 = x[i].y ^ 0x80808080u;
-                const uint32_t w2 = x[i].z ^ 0x80808080u, w3 = x[i].w ^ 0x80808080u;
                 uint8_t *d = dst + image + i * 256;
                 const int swizzle = (2 * i + odd) & 7;
                 *reinterpret_cast<uint4 *>(d + (((2 * q) ^ swizzle) << 4)) =
-                    make_uint4(fp16_codes(w0, 0x4140), fp16_codes(w0, 0x4342), fp16_codes(w1, 0x4140), fp16_codes(w1, 0x4342));
+                    fp16_codes<V>(x[i].x, x[i].y);
                 *reinterpret_cast<uint4 *>(d + (((2 * q + 1) ^ swizzle) << 4)) =
-                    make_uint4(fp16_codes(w2, 0x4140), fp16_codes(w2, 0x4342), fp16_codes(w3, 0x4140), fp16_codes(w3, 0x4342));
+                    fp16_codes<V>(x[i].z, x[i].w);
             }
         };
         // A tile of fp16 rows; rows past the last position and value rows in `skip` (new tokens, bits) are zero.
@@ -214,8 +228,9 @@ __global__ void __launch_bounds__(THREADS8, 1) attention8_kernel(const FaParams 
                 break;
             }
             if (j >= 2 && !warp_wait(empty + s, (uint32_t)((j >> 1) - 1) & 1, abort_flag)) break;
-            if (j < code_tiles) convert(dst, j);
-            else copy_rows(dst, rows, j, part && fresh ? *reinterpret_cast<volatile uint32_t *>(bad_values) : 0u);
+            if (j >= code_tiles) copy_rows(dst, rows, j, part && fresh ? *reinterpret_cast<volatile uint32_t *>(bad_values) : 0u);
+            else if (part) convert(std::true_type{}, dst, j);
+            else convert(std::false_type{}, dst, j);
             publish(full + s);                   // the slot has been read, too
             if (issued < code_tiles) {
                 if (lane == 0) fetch(issued);
@@ -270,7 +285,15 @@ __global__ void __launch_bounds__(THREADS8, 1) attention8_kernel(const FaParams 
         return;
     }
 
-    prepare_queries(p, kv_head, rope, smem + L::SM_QSTAGE, tmem, q_ready, [&] { mbar_arrive(q_loaded); });
+    // The scales of this CTA's tiles, one tile a thread: read one by one inside
+    // the loop, each tile waited for a miss in memory.
+    float k_scale = 1.f, v_scale = 1.f;
+    if ((int)threadIdx.x < code_tiles) {
+        k_scale = c.ks[(size_t)(tile0 + threadIdx.x) * NKV + kv_head];
+        v_scale = c.vs[(size_t)(tile0 + threadIdx.x) * NKV + kv_head];
+    }
+    float row_sums[QR];
+    prepare_queries<true>(p, kv_head, rope, smem + L::SM_QSTAGE, tmem, q_ready, [&] { mbar_arrive(q_loaded); }, row_sums);
     if ((warp == 2 || warp == 3) && appends) {
         const int ring = c.ring;
         const uint32_t bad = append_rows<true>(p, kv_head, warp - 2, app_lo, app_hi, rope, [ring](int pos) { return pos % ring; });
@@ -292,21 +315,27 @@ __global__ void __launch_bounds__(THREADS8, 1) attention8_kernel(const FaParams 
         float m_use[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 #pragma unroll
         for (int u = 0; u < 2; ++u) last[u] = r0 + 8 * u < rows ? p.position + (r0 + 8 * u) / GROUP : -1;
-        auto scales_of = [&](int j, float &ks, float &vs) {
-            const bool codes = j < code_tiles;
-            ks = codes ? c.ks[(size_t)(tile0 + j) * NKV + kv_head] : 1.f;
-            vs = codes ? c.vs[(size_t)(tile0 + j) * NKV + kv_head] : 1.f;
-        };
-        float ks, vs;
-        scales_of(0, ks, vs);
-        named_barrier(4, 32 * SOFT_WARPS);                         // the append has used the rotary table
+        // Once the append has used the rotary table, its place takes the queries'
+        // sums (row warp + 8 j) and the scales.
+        float *sums = maxima + 4 * DECODE_ROWS, *scales = sums + DECODE_ROWS, bias[2];
+        named_barrier(4, 32 * SOFT_WARPS);
+        if (threadIdx.x < MAX_TILES8) *reinterpret_cast<float2 *>(scales + 2 * threadIdx.x) = make_float2(k_scale, v_scale);
+        if (lane == 0)
+#pragma unroll
+            for (int i = 0; i < QR; ++i) sums[warp + 8 * i] = row_sums[i];
+        named_barrier(6, 32 * SOFT_WARPS);
+#pragma unroll
+        for (int u = 0; u < 2; ++u) bias[u] = 128.f * sums[r0 + 8 * u];
         for (int j = 0; j < ntiles; ++j) {
             const int b = j & 1;
-            const float to_log2 = SCORE_LOG2 * ks;
+            // a score in log2 units: x to_log2 + unbias
+            const bool codes = j < code_tiles;
+            const float2 scale = *reinterpret_cast<const float2 *>(scales + 2 * j);
+            const float score_log2 = SCORE_LOG2 * scale.x, to_log2 = codes ? score_log2 * KEY_UNIT : score_log2;
+            const float unbias[2] = {codes ? -bias[0] * score_log2 : 0.f, codes ? -bias[1] * score_log2 : 0.f};
             // a scale of (almost) zero: its codes count nothing, its keys still do; NaN stays
-            const float v_scale = vs < 0x1p-100f ? 0x1p-100f : vs;
-            const float v_log2 = log2f(v_scale), v_inv = 1.f / v_scale;
-            scales_of(j + 1, ks, vs);
+            const float vs = scale.y < 0x1p-100f ? 0x1p-100f : scale.y;
+            const float v_log2 = log2_approx(vs), v_inv = rcp_approx(vs);
             if (!warp_wait(s_full + b, (j >> 1) & 1, abort_flag)) break;
             tc_fence_after();
             float2 x[8];
@@ -319,7 +348,7 @@ __global__ void __launch_bounds__(THREADS8, 1) attention8_kernel(const FaParams 
                 for (int q = 0; q < 8; ++q)
                     x[q] = fadd2(make_float2(hi[2 * q], hi[2 * q + 1]), make_float2(lo[2 * q], lo[2 * q + 1]));
             }
-            if (j >= code_tiles) {                                 // only fp16 tiles hold positions past a query
+            if (!codes) {                                          // only fp16 tiles hold positions past a query
                 const int key0 = (tile0 + j) * BN + part * 32 + 2 * (lane & 3);
                 uint32_t bad = 0;
                 if (appends && (tile0 + j + 1) * BN > p.position) {
@@ -361,7 +390,7 @@ __global__ void __launch_bounds__(THREADS8, 1) attention8_kernel(const FaParams 
             bool need = false;
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
-                m[u] = fmaf(fmaxf(m[u], other[r0 + 8 * u]), to_log2, v_log2);     // log2 units (-inf stays -inf)
+                m[u] = fmaf(fmaxf(m[u], other[r0 + 8 * u]), to_log2, unbias[u] + v_log2);     // log2 units (-inf stays -inf)
                 factor[u] = 1.f;
                 if (m[u] > m_use[u] + RESCALE_THRESHOLD) {
                     factor[u] = exp2_approx(m_use[u] - m[u]);
@@ -393,7 +422,7 @@ __global__ void __launch_bounds__(THREADS8, 1) attention8_kernel(const FaParams 
             float2 shift[2], sum[2];
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
-                const float f = v_log2 + P_BIAS - (m_use[u] == -INFINITY ? 0.f : m_use[u]);
+                const float f = unbias[u] + v_log2 + P_BIAS - (m_use[u] == -INFINITY ? 0.f : m_use[u]);
                 shift[u] = make_float2(f, f);
                 sum[u] = make_float2(0.f, 0.f);
             }
@@ -418,14 +447,13 @@ __global__ void __launch_bounds__(THREADS8, 1) attention8_kernel(const FaParams 
         }
         // The rows' running max and sum, for the split combine (both warps of a
         // row moved the same maximum).
-        float *sums = maxima + 4 * DECODE_ROWS;
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
             l[u] += __shfl_xor_sync(0xffffffffu, l[u], 1);
             l[u] += __shfl_xor_sync(0xffffffffu, l[u], 2);
             if (part == 1 && (lane & 3) == 0) sums[r0 + 8 * u] = l[u];
         }
-        named_barrier(8 + wq, 64);
+        named_barrier(8 + wq, 64);         // (the queries' sums were read before the first exchange)
 #pragma unroll
         for (int u = 0; u < 2; ++u)
             if (part == 0 && (lane & 3) == 0 && r0 + 8 * u < rows) {
@@ -467,6 +495,7 @@ void attention8_run(float *out, const int8_t *kc, const float *ks, const int8_t 
     const int rows = position + T;
     const Split sp = decode_split(rows);
     if (ws_bytes < decode_parts_bytes(sp)) throw std::invalid_argument("attention workspace too small");
+    if (sp.tiles > MAX_TILES8) throw std::runtime_error("too few SMs for the 8-bit attention kernel");
     const DecodeParts parts = decode_parts(ws, sp);
     FaParams p{};
     p.q_gate = q_gate; p.out = out; p.T = T; p.position = position; p.kv_rows = rows;
