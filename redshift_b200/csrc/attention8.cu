@@ -17,10 +17,12 @@
 //    every tile, 4 KB in a row, and brings them into its own ring of three slots
 //    with one bulk copy each (96 KB in flight per SM, no barrier between warps);
 //  * the eight warps that prepared the queries are the softmax, two for each
-//    quarter of TMEM's lanes, 32 columns each.  They read their scores as 16-lane
-//    fragments, which puts the hi and lo halves of a score into the same thread,
-//    and write the probabilities back to TMEM over them, where the PV MMA reads
-//    its A operand;
+//    quarter of TMEM's lanes, which take the tiles in turn: a tile's latency from
+//    its scores to its probabilities is longer than its share of the time, and
+//    only the running maximum passes from one tile to the next.  They read their
+//    scores as 16-lane fragments, which puts the hi and lo halves of a score into
+//    the same thread, and write the probabilities back to TMEM over them, where
+//    the PV MMA reads its A operand;
 //  * a warp of its own issues the MMAs, as one (mma_f16_ts_by), which keeps the
 //    issue fast beside warps that use every slot.
 // The rest is the fp16 kernel's: queries in TMEM as fp16 hi + lo rows, a lazily
@@ -59,7 +61,7 @@ struct A8Layout {
     static constexpr int SM_BAR = SM_RAW + RAW_SLOTS * 2 * CODES_TILE;
     static constexpr int SM_ROPE = SM_BAR + 512;                  // (cos, sin) [T][32]; then maxima, sums and scales
     static constexpr int SMEM_BYTES = SM_ROPE + MAX_DECODE_T * 32 * 8;
-    static_assert((5 * DECODE_ROWS + 2 * MAX_TILES8) * 4 <= MAX_DECODE_T * 32 * 8);
+    static_assert((3 * DECODE_ROWS + 2 * MAX_TILES8) * 4 <= MAX_DECODE_T * 32 * 8);
 };
 static_assert(A8Layout::SMEM_BYTES <= 227 * 1024, "attention kernel exceeds the shared memory of a CTA");
 static_assert(EPILOGUE_BYTES <= A8Layout::SM_BAR, "O staging exceeds the images and the ring");
@@ -101,7 +103,7 @@ __global__ void __launch_bounds__(THREADS8, 1) attention8_kernel(const FaParams 
     uint64_t *raw_full = reinterpret_cast<uint64_t *>(smem + L::SM_BAR);         // [8 warps][RAW_SLOTS]
     uint64_t *k_full = raw_full + 8 * RAW_SLOTS, *v_full = k_full + 2, *k_empty = k_full + 4, *v_empty = k_full + 6,
              *s_full = k_full + 8, *p_full = k_full + 10, *p_free = k_full + 12, *mma_done = k_full + 14,
-             *q_ready = k_full + 15, *app_done = k_full + 16, *cbar = k_full + 17, *q_loaded = k_full + 18, *exchanged = k_full + 19;   // 51 in all
+             *q_ready = k_full + 15, *app_done = k_full + 16, *cbar = k_full + 17, *q_loaded = k_full + 18, *maximum_of = k_full + 19;  // 51 in all
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + L::SM_BAR + 416);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + L::SM_BAR + 420);
     uint32_t *bad_values = reinterpret_cast<uint32_t *>(smem + L::SM_BAR + 424);
@@ -125,14 +127,14 @@ __global__ void __launch_bounds__(THREADS8, 1) attention8_kernel(const FaParams 
         for (int i = 0; i < 2; ++i) {
             mbar_init(k_full + i, CONV_WARPS); mbar_init(v_full + i, CONV_WARPS);
             mbar_init(k_empty + i, 1); mbar_init(v_empty + i, 1);
-            mbar_init(s_full + i, 1); mbar_init(p_full + i, SOFT_WARPS); mbar_init(p_free + i, 1);
+            mbar_init(s_full + i, 1); mbar_init(p_full + i, SOFT_WARPS / 2); mbar_init(p_free + i, 1);
         }
         mbar_init(mma_done, 1);
         mbar_init(q_ready, 8);
         mbar_init(cbar, 1);
         mbar_init(app_done, 64);
         mbar_init(q_loaded, 1);
-        for (int i = 0; i < 8; ++i) mbar_init(exchanged + i, 2);
+        for (int i = 0; i < 8; ++i) mbar_init(maximum_of + i, 1);
         *abort_flag = 0;
         *bad_values = 0;
         fence_barrier_init();
@@ -304,20 +306,20 @@ __global__ void __launch_bounds__(THREADS8, 1) attention8_kernel(const FaParams 
     {
         // ------------------------------------------------ softmax
         // Lanes 32g + i and 32g + 16 + i of TMEM hold the hi and lo halves of query
-        // row 16g + i.  Warp w has the rows of g = w % 4 and the columns 32 (w / 4)
-        // to + 32 of every tile; thread l of it the rows 16g + l / 4 + 8 u (u = 0,
-        // 1) and, of these, the columns 8 n + 2 (l % 4) + e in x[2 n + u].
-        const int wq = warp & 3, part = warp >> 2;
+        // row 16g + i.  Warps g and g + 4 have the rows of g, the first in the even
+        // tiles, the second in the odd ones; thread l of them the rows 16g + l / 4 +
+        // 8 u (u = 0, 1) and, of these, the columns 8 n + 2 (l % 4) + e in x[2 n + u].
+        const int wq = warp & 3, turn = warp >> 2;
         const uint32_t t_hi = tmem + ((uint32_t)(wq * 32) << 16), t_lo = t_hi + (16u << 16);
         const int r0 = wq * 16 + (lane >> 2), rows = p.T * GROUP;
-        float *maxima = reinterpret_cast<float *>(rope);           // [tile parity][part][64 rows], once the rotary table is used up
         int last[2];                                               // last visible position
         float m_use[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 #pragma unroll
         for (int u = 0; u < 2; ++u) last[u] = r0 + 8 * u < rows ? p.position + (r0 + 8 * u) / GROUP : -1;
         // Once the append has used the rotary table, its place takes the queries'
-        // sums (row warp + 8 j) and the scales.
-        float *sums = maxima + 4 * DECODE_ROWS, *scales = sums + DECODE_ROWS, bias[2];
+        // sums (row warp + 8 j), the scales and the running maxima.
+        float *maxima = reinterpret_cast<float *>(rope);           // [tile parity][64 rows]
+        float *sums = maxima + 2 * DECODE_ROWS, *scales = sums + DECODE_ROWS, bias[2];
         named_barrier(4, 32 * SOFT_WARPS);
         if (threadIdx.x < MAX_TILES8) *reinterpret_cast<float2 *>(scales + 2 * threadIdx.x) = make_float2(k_scale, v_scale);
         if (lane == 0)
@@ -326,30 +328,30 @@ __global__ void __launch_bounds__(THREADS8, 1) attention8_kernel(const FaParams 
         named_barrier(6, 32 * SOFT_WARPS);
 #pragma unroll
         for (int u = 0; u < 2; ++u) bias[u] = 128.f * sums[r0 + 8 * u];
-        for (int j = 0; j < ntiles; ++j) {
-            const int b = j & 1;
+        for (int j = turn; j < ntiles; j += 2) {
+            const int b = turn;
             // a score in log2 units: x to_log2 + unbias
             const bool codes = j < code_tiles;
             const float2 scale = *reinterpret_cast<const float2 *>(scales + 2 * j);
             const float score_log2 = SCORE_LOG2 * scale.x, to_log2 = codes ? score_log2 * KEY_UNIT : score_log2;
-            const float unbias[2] = {codes ? -bias[0] * score_log2 : 0.f, codes ? -bias[1] * score_log2 : 0.f};
             // a scale of (almost) zero: its codes count nothing, its keys still do; NaN stays
             const float vs = scale.y < 0x1p-100f ? 0x1p-100f : scale.y;
             const float v_log2 = log2_approx(vs), v_inv = rcp_approx(vs);
             if (!warp_wait(s_full + b, (j >> 1) & 1, abort_flag)) break;
             tc_fence_after();
-            float2 x[8];
-            {
+            float2 x[16];
+#pragma unroll
+            for (int part = 0; part < 2; ++part) {
                 float hi[16], lo[16];
                 tmem_ld_16x256b_x4(t_hi + TM_S + b * BN + part * 32, hi);
                 tmem_ld_16x256b_x4(t_lo + TM_S + b * BN + part * 32, lo);
                 tmem_wait_ld();
 #pragma unroll
                 for (int q = 0; q < 8; ++q)
-                    x[q] = fadd2(make_float2(hi[2 * q], hi[2 * q + 1]), make_float2(lo[2 * q], lo[2 * q + 1]));
+                    x[8 * part + q] = fadd2(make_float2(hi[2 * q], hi[2 * q + 1]), make_float2(lo[2 * q], lo[2 * q + 1]));
             }
             if (!codes) {                                          // only fp16 tiles hold positions past a query
-                const int key0 = (tile0 + j) * BN + part * 32 + 2 * (lane & 3);
+                const int key0 = (tile0 + j) * BN + 2 * (lane & 3);
                 uint32_t bad = 0;
                 if (appends && (tile0 + j + 1) * BN > p.position) {
                     if (!warp_wait(app_done, 0, abort_flag)) break;
@@ -364,49 +366,51 @@ __global__ void __launch_bounds__(THREADS8, 1) attention8_kernel(const FaParams 
                     return key <= last[u] ? v : -INFINITY;
                 };
 #pragma unroll
-                for (int q = 0; q < 8; ++q) {
+                for (int q = 0; q < 16; ++q) {
                     x[q].x = masked(x[q].x, key0 + 8 * (q >> 1), q & 1);
                     x[q].y = masked(x[q].y, key0 + 8 * (q >> 1) + 1, q & 1);
                 }
             }
-            // The row's maximum: this thread's columns, the row's other three
-            // threads, and the warp with the other 32 columns.  Behind the exchange
-            // both warps have read their scores, so P may overwrite them.
-            float m[2], factor[2];
-            float *mine = maxima + (b * 2 + part) * DECODE_ROWS, *other = maxima + (b * 2 + 1 - part) * DECODE_ROWS;
+            // The row's maximum: this thread's columns and the row's other three threads.
+            float m[2], before[2] = {-INFINITY, -INFINITY}, unbias[2];
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
-                m[u] = fmaxf(fmaxf(fmaxf(x[u].x, x[u].y), fmaxf(x[2 + u].x, x[2 + u].y)),
-                             fmaxf(fmaxf(x[4 + u].x, x[4 + u].y), fmaxf(x[6 + u].x, x[6 + u].y)));
+                float m0 = fmaxf(x[u].x, x[u].y), m1 = fmaxf(x[2 + u].x, x[2 + u].y);
+#pragma unroll
+                for (int n = 2; n < 8; n += 2) {
+                    m0 = fmaxf(m0, fmaxf(x[2 * n + u].x, x[2 * n + u].y));
+                    m1 = fmaxf(m1, fmaxf(x[2 * n + 2 + u].x, x[2 * n + 2 + u].y));
+                }
+                m[u] = fmaxf(m0, m1);
                 m[u] = fmaxf(m[u], __shfl_xor_sync(0xffffffffu, m[u], 1));
                 m[u] = fmaxf(m[u], __shfl_xor_sync(0xffffffffu, m[u], 2));
-                if ((lane & 3) == 0) mine[r0 + 8 * u] = m[u];
+                unbias[u] = codes ? -bias[u] * score_log2 : 0.f;
+                m[u] = fmaf(m[u], to_log2, unbias[u] + v_log2);    // log2 units (-inf stays -inf)
             }
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(exchanged + 2 * wq + b);
-            if (!warp_wait(exchanged + 2 * wq + b, (j >> 1) & 1, abort_flag)) break;
-            tc_fence_after();
+            // The running maximum of the tile before, from this row's other warp; it
+            // moves only when the tile's is far above it.
+            if (j > 0) {
+                if (!warp_wait(maximum_of + 2 * wq + (b ^ 1), ((j - 1) >> 1) & 1, abort_flag)) break;
+#pragma unroll
+                for (int u = 0; u < 2; ++u) before[u] = maxima[(b ^ 1) * DECODE_ROWS + r0 + 8 * u];
+            }
             bool need = false;
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
-                m[u] = fmaf(fmaxf(m[u], other[r0 + 8 * u]), to_log2, unbias[u] + v_log2);     // log2 units (-inf stays -inf)
-                factor[u] = 1.f;
-                if (m[u] > m_use[u] + RESCALE_THRESHOLD) {
-                    factor[u] = exp2_approx(m_use[u] - m[u]);
-                    m_use[u] = m[u];
-                    l[u] *= factor[u];
-                    need = true;
-                }
+                const bool raise = m[u] > before[u] + RESCALE_THRESHOLD;
+                need = need || raise;
+                m[u] = raise ? m[u] : before[u];
             }
             if (j > 0 && __any_sync(0xffffffffu, need)) {
-                // O already holds tiles < j: wait for PV(j-1), then rescale its rows
-                // (this warp's half of the columns).
-                if (!warp_wait(p_free + ((j - 1) & 1), ((j - 1) >> 1) & 1, abort_flag)) break;
+                // O holds the tiles before j: wait for PV(j-1), then rescale its rows.
+                if (!warp_wait(p_free + (b ^ 1), ((j - 1) >> 1) & 1, abort_flag)) break;
                 tc_fence_after();
+                float factor[2];
+#pragma unroll
+                for (int u = 0; u < 2; ++u) factor[u] = m[u] == before[u] ? 1.f : exp2_approx(before[u] - m[u]);
 #pragma unroll 1
-                for (int q = 0; q < HD / 32; ++q) {
-                    const uint32_t at = (q & 1 ? t_lo : t_hi) + TM_O + part * (HD / 2) + (q >> 1) * 32;
+                for (int q = 0; q < 2 * HD / 32; ++q) {
+                    const uint32_t at = (q & 1 ? t_lo : t_hi) + TM_O + (q >> 1) * 32;
                     float o[16];
                     uint32_t scaled[16];
                     tmem_ld_16x256b_x4(at, o);
@@ -416,50 +420,70 @@ __global__ void __launch_bounds__(THREADS8, 1) attention8_kernel(const FaParams 
                     tmem_st_16x256b_x4(at, scaled);
                 }
                 tmem_wait_st();
+                tc_fence_before();
             }
-            uint32_t hi[8], lo[8];
+            if ((lane & 3) == 0) {
+#pragma unroll
+                for (int u = 0; u < 2; ++u) maxima[b * DECODE_ROWS + r0 + 8 * u] = m[u];
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(maximum_of + 2 * wq + b);
             const float2 scale2 = make_float2(to_log2, to_log2), minus = make_float2(-1.f, -1.f);
             float2 shift[2], sum[2];
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
+                if (m[u] != m_use[u]) {                            // moved since this warp's last tile
+                    l[u] *= exp2_approx(m_use[u] - m[u]);
+                    m_use[u] = m[u];
+                }
                 const float f = unbias[u] + v_log2 + P_BIAS - (m_use[u] == -INFINITY ? 0.f : m_use[u]);
                 shift[u] = make_float2(f, f);
                 sum[u] = make_float2(0.f, 0.f);
             }
 #pragma unroll
-            for (int q = 0; q < 8; ++q) {
-                const float2 arg = ffma2(x[q], scale2, shift[q & 1]);
-                const float2 e = make_float2(exp2_approx(arg.x), exp2_approx(arg.y));
-                sum[q & 1] = fadd2(sum[q & 1], e);
-                const __half2 h = __floats2half2_rn(e.x, e.y);
-                hi[q] = half2_bits(h);
-                const float2 rest = ffma2(__half22float2(h), minus, e);
-                lo[q] = half2_bits(__floats2half2_rn(rest.x, rest.y));
+            for (int part = 0; part < 2; ++part) {
+                uint32_t hi[8], lo[8];
+#pragma unroll
+                for (int q = 0; q < 8; ++q) {
+                    const float2 arg = ffma2(x[8 * part + q], scale2, shift[q & 1]);
+                    const float2 e = make_float2(exp2_approx(arg.x), exp2_approx(arg.y));
+                    sum[q & 1] = fadd2(sum[q & 1], e);
+                    const __half2 h = __floats2half2_rn(e.x, e.y);
+                    hi[q] = half2_bits(h);
+                    const float2 rest = ffma2(__half22float2(h), minus, e);
+                    lo[q] = half2_bits(__floats2half2_rn(rest.x, rest.y));
+                }
+                tmem_st_16x128b_x4(t_hi + TM_S + b * BN + part * 16, hi);
+                tmem_st_16x128b_x4(t_lo + TM_S + b * BN + part * 16, lo);
             }
 #pragma unroll
             for (int u = 0; u < 2; ++u) l[u] = fmaf(sum[u].x + sum[u].y, v_inv, l[u]);
-            tmem_st_16x128b_x4(t_hi + TM_S + b * BN + part * 16, hi);
-            tmem_st_16x128b_x4(t_lo + TM_S + b * BN + part * 16, lo);
             tmem_wait_st();
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(p_full + b);
         }
-        // The rows' running max and sum, for the split combine (both warps of a
-        // row moved the same maximum).
+        // The rows' maximum and sum, for the split combine: the last tile's warp has
+        // the final maximum, the other brings its sum to it.
+        float *finals = maxima + 2 * DECODE_ROWS;                  // (max, sum) [64], over the queries' sums and the scales
+        const bool ends = turn == ((ntiles - 1) & 1);
+        named_barrier(4, 32 * SOFT_WARPS);
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
             l[u] += __shfl_xor_sync(0xffffffffu, l[u], 1);
             l[u] += __shfl_xor_sync(0xffffffffu, l[u], 2);
-            if (part == 1 && (lane & 3) == 0) sums[r0 + 8 * u] = l[u];
+            if (!ends && (lane & 3) == 0)
+                *reinterpret_cast<float2 *>(finals + 2 * (r0 + 8 * u)) = make_float2(m_use[u], l[u]);
         }
-        named_barrier(8 + wq, 64);         // (the queries' sums were read before the first exchange)
+        named_barrier(8 + wq, 64);
 #pragma unroll
         for (int u = 0; u < 2; ++u)
-            if (part == 0 && (lane & 3) == 0 && r0 + 8 * u < rows) {
+            if (ends && (lane & 3) == 0 && r0 + 8 * u < rows) {
+                const float2 o = *reinterpret_cast<const float2 *>(finals + 2 * (r0 + 8 * u));
+                const float w = o.x == m_use[u] ? 1.f : exp2_approx(o.x - m_use[u]);
                 const size_t slot = ((size_t)kv_head * DECODE_ROWS + r0 + 8 * u) * MAXS + blockIdx.x;
                 p.part_ml[slot * 2] = m_use[u];
-                p.part_ml[slot * 2 + 1] = l[u] + sums[r0 + 8 * u];
+                p.part_ml[slot * 2 + 1] = fmaf(o.y, w, l[u]);
             }
     }
     // The final PV's commit on p_free marks O complete and every image consumed.
