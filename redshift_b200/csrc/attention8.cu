@@ -13,9 +13,9 @@
 // Bound by the cache's bytes, 2 KB a position.  What keeps the tensor cores fed
 // at twice the fp16 cache's tile rate:
 //  * eight converter warps (four for K, four for V) write the codes as exact fp16
-//    integers into the MMA's swizzled operand images.  A warp owns 16 rows of
-//    every tile, 4 KB in a row, and brings them into its own ring of three slots
-//    with one bulk copy each (96 KB in flight per SM, no barrier between warps);
+//    numbers into the MMA's swizzled operand images.  A producer warp keeps three
+//    tiles of K and of V on their way in shared memory (96 KB per SM; a block of
+//    one head is 16 KB in a row, one bulk copy);
 //  * the eight warps that prepared the queries are the softmax, two for each
 //    quarter of TMEM's lanes, which take the tiles in turn: a tile's latency from
 //    its scores to its probabilities is longer than its share of the time, and
@@ -48,8 +48,9 @@ namespace {
 
 constexpr int IMAGES = 2;        // fp16 tile images (K and V each)
 constexpr int RAW_SLOTS = 3;     // code tiles in flight (K and V each)
-constexpr int WARP_ROWS = 16, WARP_BYTES = WARP_ROWS * HD;        // a converter warp's part of a code tile
-constexpr int SOFT_WARPS = 8, CONV_WARPS = 4, THREADS8 = 32 * (SOFT_WARPS + 2 * CONV_WARPS + 1);
+constexpr int WARP_ROWS = 16;    // a converter warp's rows of a tile
+constexpr int SOFT_WARPS = 8, CONV_WARPS = 4, MMA_WARP = SOFT_WARPS + 2 * CONV_WARPS, PRODUCER_WARP = MMA_WARP + 1;
+constexpr int THREADS8 = 32 * (PRODUCER_WARP + 1);
 constexpr int CODES_TILE = BN * HD;                               // codes of one (block, head)
 constexpr int MAX_TILES8 = 160;  // tiles of a CTA (59 at the longest context on 148 SMs)
 constexpr float P_BIAS = 6.f;    // log2 units above the running maximum
@@ -59,7 +60,7 @@ struct A8Layout {
     static constexpr int SM_RAW = SM_KV + IMAGES * SM_KV_STAGE;   // code tiles [slot][K, V]
     static constexpr int SM_QSTAGE = SM_RAW + 4 * CODES_TILE;     // slot 2 until the queries are in TMEM
     static constexpr int SM_BAR = SM_RAW + RAW_SLOTS * 2 * CODES_TILE;
-    static constexpr int SM_ROPE = SM_BAR + 512;                  // (cos, sin) [T][32]; then maxima, sums and scales
+    static constexpr int SM_ROPE = SM_BAR + 384;                  // (cos, sin) [T][32]; then maxima, sums and scales
     static constexpr int SMEM_BYTES = SM_ROPE + MAX_DECODE_T * 32 * 8;
     static_assert((3 * DECODE_ROWS + 2 * MAX_TILES8) * 4 <= MAX_DECODE_T * 32 * 8);
 };
@@ -100,13 +101,13 @@ __global__ void __launch_bounds__(THREADS8, 1) attention8_kernel(const FaParams 
         if (threadIdx.x == 0) raise_status(STATUS_BAD_ARGUMENT);
         return;
     }
-    uint64_t *raw_full = reinterpret_cast<uint64_t *>(smem + L::SM_BAR);         // [8 warps][RAW_SLOTS]
-    uint64_t *k_full = raw_full + 8 * RAW_SLOTS, *v_full = k_full + 2, *k_empty = k_full + 4, *v_empty = k_full + 6,
+    uint64_t *raw_full = reinterpret_cast<uint64_t *>(smem + L::SM_BAR), *raw_empty = raw_full + 2 * RAW_SLOTS;   // [K, V][slot]
+    uint64_t *k_full = raw_empty + 2 * RAW_SLOTS, *v_full = k_full + 2, *k_empty = k_full + 4, *v_empty = k_full + 6,
              *s_full = k_full + 8, *p_full = k_full + 10, *p_free = k_full + 12, *mma_done = k_full + 14,
-             *q_ready = k_full + 15, *app_done = k_full + 16, *cbar = k_full + 17, *q_loaded = k_full + 18, *maximum_of = k_full + 19;  // 51 in all
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + L::SM_BAR + 416);
-    volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + L::SM_BAR + 420);
-    uint32_t *bad_values = reinterpret_cast<uint32_t *>(smem + L::SM_BAR + 424);
+             *q_ready = k_full + 15, *app_done = k_full + 16, *cbar = k_full + 17, *q_loaded = k_full + 18, *maximum_of = k_full + 19;  // 39 in all
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + L::SM_BAR + 320);
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + L::SM_BAR + 324);
+    uint32_t *bad_values = reinterpret_cast<uint32_t *>(smem + L::SM_BAR + 328);
     float2 *rope = reinterpret_cast<float2 *>(smem + L::SM_ROPE);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -123,7 +124,7 @@ __global__ void __launch_bounds__(THREADS8, 1) attention8_kernel(const FaParams 
         prefetch_l2(p.q_gate + ((size_t)(rr / GROUP) * NQ + kv_head * GROUP + rr % GROUP) * 2 * HD + (i & 7) * 32);
     }
     if (threadIdx.x == 0) {
-        for (int i = 0; i < 8 * RAW_SLOTS; ++i) mbar_init(raw_full + i, 1);
+        for (int i = 0; i < 2 * RAW_SLOTS; ++i) { mbar_init(raw_full + i, 1); mbar_init(raw_empty + i, CONV_WARPS); }
         for (int i = 0; i < 2; ++i) {
             mbar_init(k_full + i, CONV_WARPS); mbar_init(v_full + i, CONV_WARPS);
             mbar_init(k_empty + i, 1); mbar_init(v_empty + i, 1);
@@ -149,7 +150,7 @@ __global__ void __launch_bounds__(THREADS8, 1) attention8_kernel(const FaParams 
 
     const int code_tiles = max(0, min(ntiles, c.blocks - tile0));       // tiles of codes, the first of this CTA's
 
-    if (warp >= SOFT_WARPS && warp < SOFT_WARPS + 2 * CONV_WARPS) {
+    if (warp >= SOFT_WARPS && warp < MMA_WARP) {
         // ------------------------------------------------ converters (warps 8-11: K, 12-15: V)
         // A lane takes 16 codes (16 dims of a row) at a time: 16 bytes of the
         // code tile, two 16-byte chunks of a 64-dim box of the image.  Eight
@@ -160,19 +161,12 @@ __global__ void __launch_bounds__(THREADS8, 1) attention8_kernel(const FaParams 
         const int part = (warp - SOFT_WARPS) >> 2, w = warp & 3, q = lane & 3, odd = lane >> 2 & 1;
         const int box = (lane >> 3) ^ odd, piece = 4 * box + q, row0 = WARP_ROWS * w + odd;
         const uint32_t image = box * (BN * 128) + row0 * 128;
-        const int8_t *codes = (part ? c.vc : c.kc) + ((size_t)tile0 * NKV + kv_head) * CODES_TILE + w * WARP_BYTES;
-        uint8_t *ring = smem + L::SM_RAW + part * CODES_TILE + w * WARP_BYTES;
-        uint64_t *landed = raw_full + (warp - SOFT_WARPS) * RAW_SLOTS;
-        int issued = 0;
-        auto fetch = [&](int j) {                               // one lane: tile j's rows of this warp
-            const int slot = j % RAW_SLOTS;
-            mbar_expect_tx(landed + slot, WARP_BYTES);
-            bulk_load(ring + slot * 2 * CODES_TILE, codes + (size_t)j * (NKV * CODES_TILE), WARP_BYTES, landed + slot);
-        };
-        auto convert = [&](auto values, uint8_t *dst, int j) {
+        const uint8_t *ring = smem + L::SM_RAW + part * CODES_TILE + row0 * HD + piece * 16;
+        uint64_t *landed = raw_full + part * RAW_SLOTS, *taken = raw_empty + part * RAW_SLOTS;
+        auto convert = [&](auto values, uint8_t *dst, int slot) {
             constexpr bool V = decltype(values)::value;
             uint4 x[8];
-            const uint8_t *src = ring + j % RAW_SLOTS * 2 * CODES_TILE + odd * HD + piece * 16;
+            const uint8_t *src = ring + slot * 2 * CODES_TILE;
 #pragma unroll
             for (int i = 0; i < 8; ++i) x[i] = *reinterpret_cast<const uint4 *>(src + i * 2 * HD);
 #pragma unroll
@@ -209,44 +203,62 @@ __global__ void __launch_bounds__(THREADS8, 1) attention8_kernel(const FaParams 
         };
         uint64_t *full = part ? v_full : k_full, *empty = part ? v_empty : k_empty;
         const __half *rows = part ? p.vc : p.kc;
-        // The first copies go out once the query rows have arrived (issued before
-        // them they would queue in front), the last slot once it stages no queries.
-        if (code_tiles > 0 && warp_wait(q_loaded, 0, abort_flag)) {
-            issued = min(code_tiles, RAW_SLOTS - 1);
-            if (lane == 0) for (int j = 0; j < issued; ++j) fetch(j);
-            if (issued < code_tiles && warp_wait(q_ready, 0, abort_flag)) {
-                fence_async_shared();            // the staged queries were written and read by plain accesses
-                if (lane == 0) fetch(issued);
-                ++issued;
-            }
-        }
-        for (int j = 0; j < ntiles; ++j) {
+        for (int j = 0, slot = 0, lap = 0; j < ntiles; ++j) {
             const int s = j & 1;
             uint8_t *dst = smem + L::SM_KV + s * L::SM_KV_STAGE + part * TILE_BYTES;
             const bool fresh = appends && (tile0 + j + 1) * BN > p.position;      // the tile holds new rows
             if (j < code_tiles) {
-                if (!warp_wait(landed + j % RAW_SLOTS, (uint32_t)(j / RAW_SLOTS) & 1, abort_flag)) break;
+                if (!warp_wait(landed + slot, lap & 1, abort_flag)) break;
             } else if (fresh && !warp_wait(app_done, 0, abort_flag)) {
                 break;
             }
             if (j >= 2 && !warp_wait(empty + s, (uint32_t)((j >> 1) - 1) & 1, abort_flag)) break;
             if (j >= code_tiles) copy_rows(dst, rows, j, part && fresh ? *reinterpret_cast<volatile uint32_t *>(bad_values) : 0u);
-            else if (part) convert(std::true_type{}, dst, j);
-            else convert(std::false_type{}, dst, j);
-            publish(full + s);                   // the slot has been read, too
-            if (issued < code_tiles) {
-                if (lane == 0) fetch(issued);
-                ++issued;
-            }
+            else if (part) convert(std::true_type{}, dst, slot);
+            else convert(std::false_type{}, dst, slot);
+            publish(full + s);
+            if (j < code_tiles && lane == 0) mbar_arrive(taken + slot);
+            if (++slot == RAW_SLOTS) { slot = 0; ++lap; }
         }
-        // Every issued copy must land before the CTA may exit.
-        const long long t0 = clock64();
-        for (int j = max(0, issued - RAW_SLOTS); j < issued; ++j)
-            while (!mbar_try_wait(landed + j % RAW_SLOTS, (uint32_t)(j / RAW_SLOTS) & 1) && clock64() - t0 < WAIT_LIMIT_CYCLES) {}
         return;                          // the later barriers count the first eight warps
     }
 
-    if (warp == SOFT_WARPS + 2 * CONV_WARPS) {
+    if (warp == PRODUCER_WARP) {
+        // ------------------------------------------------ producer
+        if (lane == 0 && code_tiles > 0) {
+            const size_t first = ((size_t)tile0 * NKV + kv_head) * CODES_TILE, step = (size_t)NKV * CODES_TILE;
+            const int8_t *src[2] = {c.kc + first, c.vc + first};
+            int issued = 0;                                   // halves: tile j's K is 2 j, its V 2 j + 1
+            // The first two tiles are asked for once the query rows have arrived
+            // (issued before them they would queue in front), the last slot once
+            // it stages no queries.
+            bool ok = mbar_wait(q_loaded, 0, abort_flag);
+            for (int j = 0, slot = 0, lap = 0; j < code_tiles && ok; ++j) {
+                if (j == RAW_SLOTS - 1) {
+                    ok = mbar_wait(q_ready, 0, abort_flag);
+                    fence_async_shared();                     // the staged queries were written and read by plain accesses
+                }
+#pragma unroll
+                for (int part = 0; part < 2; ++part) {
+                    uint64_t *bar = raw_full + part * RAW_SLOTS + slot;
+                    if (j >= RAW_SLOTS) ok = ok && mbar_wait(raw_empty + part * RAW_SLOTS + slot, (lap - 1) & 1, abort_flag);
+                    if (!ok) break;
+                    mbar_expect_tx(bar, CODES_TILE);
+                    bulk_load(smem + L::SM_RAW + (slot * 2 + part) * CODES_TILE, src[part], CODES_TILE, bar);
+                    src[part] += step;
+                    ++issued;
+                }
+                if (++slot == RAW_SLOTS) { slot = 0; ++lap; }
+            }
+            // Every issued copy must land before the CTA may exit.
+            const long long t0 = clock64();
+            for (int h = max(0, issued - 2 * RAW_SLOTS); h < issued; ++h)
+                while (!mbar_try_wait(raw_full + (h & 1) * RAW_SLOTS + (h >> 1) % RAW_SLOTS, (uint32_t)((h >> 1) / RAW_SLOTS) & 1) &&
+                       clock64() - t0 < WAIT_LIMIT_CYCLES) {}
+        }
+        return;
+    }
+    if (warp == MMA_WARP) {
         // ------------------------------------------------ MMA issuer (the whole warp, one elected lane)
         const uint32_t lead = elect_lane(), tm = __shfl_sync(0xffffffffu, tmem, 0);
         const uint32_t idesc_qk = idesc_f16(128, BN, false, false), idesc_pv = idesc_f16(128, HD, false, true);
