@@ -30,13 +30,14 @@ namespace {
 constexpr int KB = 128;                        // columns of a block = one 128-byte swizzled row of codes
 constexpr int ROWS = 128;                      // weight rows that share a scale
 
-// D[tmem] (+)= A[smem] * B[smem]^T for e4m3 codes, fp32 accumulate, K = 32.
-__device__ __forceinline__ void mma_e4m3_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
-                                            uint32_t accumulate) {
-    asm volatile("{\n\t.reg .pred p;\n\t"
-                 "setp.ne.b32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
-                 :: "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate) : "memory");
+// D[tmem] (+)= A[smem] * B[smem]^T for e4m3 codes, fp32 accumulate, K = 32;
+// issued by a whole warp, one elected lane (see mma_f16_ss_by).
+__device__ __forceinline__ void mma_e4m3_ss_by(uint32_t elected, uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
+                                               uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p, q;\n\t"
+                 "setp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+                 "@q tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+                 :: "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(elected) : "memory");
 }
 // Instruction descriptor: e4m3 operands (format 0 of kind::f8f6f4), both K-major, fp32 accumulator.
 __host__ __device__ constexpr uint32_t idesc_e4m3(int M, int N) {
@@ -59,6 +60,18 @@ __device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
     asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
     return v;
 }
+// The shared address of this CTA's `addr` in CTA `rank` of the cluster.
+__device__ __forceinline__ uint32_t cluster_rank(uint32_t addr, uint32_t rank) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+    return v;
+}
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
@@ -73,11 +86,12 @@ struct Mm8Params {
 
 // ---------------------------------------------------------------- few tokens
 template <int NT> struct Few {
-    // Two CTAs per SM up to 64 tokens (their rings hold 2 x 90..108 KB in
-    // flight, enough for the HBM latency), one at 128.
-    static constexpr int STAGES = NT == 16 ? 6 : NT == 32 ? 5 : NT == 64 ? 4 : 6;
+    // Two CTAs per SM: their rings hold 2 x 96..108 KB in flight, enough for the
+    // HBM latency.  Four warps scale and add up to 32 tokens, eight beyond.
+    static constexpr int STAGES = NT == 16 ? 6 : NT == 32 ? 5 : NT == 64 ? 4 : 3;
     static constexpr int BUFS = NT <= 32 ? 4 : 2;            // TMEM accumulators
-    static constexpr int CTAS = NT <= 64 ? 2 : 1;
+    static constexpr int SUM_WARPS = NT <= 32 ? 4 : 8, COLS = NT * 4 / SUM_WARPS;   // columns of a warp
+    static constexpr int THREADS = 64 + 32 * SUM_WARPS;
     static constexpr int SLOTS = STAGES + BUFS;              // scale slots
     static constexpr int W_BYTES = ROWS * KB, X_BYTES = NT * KB, STAGE = W_BYTES + X_BYTES;
     static constexpr int SLOT_FLOATS = NT + 4;
@@ -89,7 +103,7 @@ template <int NT> struct Few {
 };
 
 template <int NT>
-__global__ void __launch_bounds__(192, Few<NT>::CTAS)
+__global__ void __launch_bounds__(Few<NT>::THREADS, 2)
 few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX, const Mm8Params p) {
     using L = Few<NT>;
     extern __shared__ __align__(1024) uint8_t smem[];
@@ -108,7 +122,7 @@ few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUte
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < L::STAGES; ++i) { mbar_init(full + i, 1); mbar_init(empty + i, 1); }
-        for (int i = 0; i < L::BUFS; ++i) { mbar_init(d_full + i, 1); mbar_init(d_empty + i, 4); }
+        for (int i = 0; i < L::BUFS; ++i) { mbar_init(d_full + i, 1); mbar_init(d_empty + i, L::SUM_WARPS); }
         for (int i = 0; i < L::SLOTS; ++i) mbar_init(s_full + i, 32);
         mbar_init(mma_done, 1);
         *abort_flag = bad_base ? 1 : 0;
@@ -125,9 +139,10 @@ few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUte
     grid_dependency_wait();
     if (threadIdx.x == 0) launch_dependents();
 
-    float acc[NT];
+    float2 acc[L::COLS / 2];
 #pragma unroll
-    for (int c = 0; c < NT; ++c) acc[c] = 0.f;
+    for (int c = 0; c < L::COLS / 2; ++c) acc[c] = make_float2(0.f, 0.f);
+    const int col0 = (warp - 2) / 4 * L::COLS;                 // this warp's tokens of the tile
     bool ok = !bad_base;
     if (warp == 0) {
         // ------------------------------------------------ producer: code tiles by TMA, scales by small copies
@@ -161,47 +176,46 @@ few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUte
         }
     } else if (warp == 1) {
         // ------------------------------------------------ MMA issuer
-        if (lane == 0) {
-            constexpr uint32_t idesc = idesc_e4m3(ROWS, NT);
-            for (int j = 0; j < n && ok; ++j) {
-                const int s = j % L::STAGES, d = j % L::BUFS;
-                if (!mbar_wait(full + s, (j / L::STAGES) & 1, abort_flag)) { ok = false; break; }
-                if (j >= L::BUFS && !mbar_wait(d_empty + d, (j / L::BUFS - 1) & 1, abort_flag)) { ok = false; break; }
-                tc_fence_after();
-                const uint32_t w = smem_addr(smem + s * L::STAGE), x = w + L::W_BYTES;
+        constexpr uint32_t idesc = idesc_e4m3(ROWS, NT);
+        const uint32_t lead = elect_lane(), tm = __shfl_sync(0xffffffffu, tmem, 0);
+        for (int j = 0, s = 0, d = 0, lap = 0, dlap = 0; j < n && ok; ++j) {
+            if (!warp_wait8(full + s, lap & 1, abort_flag)) { ok = false; break; }
+            if (j >= L::BUFS && !warp_wait8(d_empty + d, (dlap - 1) & 1, abort_flag)) { ok = false; break; }
+            tc_fence_after();
+            const uint64_t w = sw128_desc(smem_addr(smem + s * L::STAGE), 16, 1024);
+            const uint64_t x = sw128_desc(smem_addr(smem + s * L::STAGE + L::W_BYTES), 16, 1024);
 #pragma unroll
-                for (int k = 0; k < KB / 32; ++k)
-                    mma_e4m3_ss(tmem + d * NT, sw128_desc(w + k * 32, 16, 1024), sw128_desc(x + k * 32, 16, 1024), idesc,
-                                k > 0 ? 1u : 0u);
-                mma_commit(empty + s);
-                mma_commit(d_full + d);
-            }
-            mma_commit(mma_done);
-            const long long start = clock64();
-            while (!mbar_try_wait(mma_done, 0) && clock64() - start < WAIT_LIMIT_CYCLES) {}
+            for (int k = 0; k < KB / 32; ++k)
+                mma_e4m3_ss_by(lead, tm + d * NT, w + 2 * k, x + 2 * k, idesc, k > 0 ? 1u : 0u);
+            mma_commit_by(lead, empty + s);
+            mma_commit_by(lead, d_full + d);
+            if (++s == L::STAGES) { s = 0; ++lap; }
+            if (++d == L::BUFS) { d = 0; ++dlap; }
         }
+        mma_commit_by(lead, mma_done);
+        const long long start = clock64();
+        while (!mbar_try_wait(mma_done, 0) && clock64() - start < WAIT_LIMIT_CYCLES) {}
     } else {
         // ------------------------------------------------ scales and sums: thread = TMEM lane = weight row
-        const uint32_t t_lane = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+        const uint32_t t_lane = tmem + ((uint32_t)((warp & 3) * 32) << 16) + col0;
         for (int j = 0; j < n; ++j) {
             const int d = j % L::BUFS, slot = j % L::SLOTS;
             if (!warp_wait8(s_full + slot, (j / L::SLOTS) & 1, abort_flag) ||
                 !warp_wait8(d_full + d, (j / L::BUFS) & 1, abort_flag)) { ok = false; break; }
             tc_fence_after();
             const float *sc = slots + slot * L::SLOT_FLOATS;
-            const float ws = sc[NT];
+            const float2 ws = make_float2(sc[NT], sc[NT]);
 #pragma unroll
-            for (int c0 = 0; c0 < NT; c0 += 16) {
+            for (int c0 = 0; c0 < L::COLS; c0 += 16) {
                 float x[16];
                 tmem_ld16(t_lane + d * NT + c0, x);
                 tmem_wait_ld();
 #pragma unroll
                 for (int c = 0; c < 16; c += 4) {
-                    const float4 f = *reinterpret_cast<const float4 *>(sc + c0 + c);
-                    acc[c0 + c] = fmaf(x[c], f.x * ws, acc[c0 + c]);
-                    acc[c0 + c + 1] = fmaf(x[c + 1], f.y * ws, acc[c0 + c + 1]);
-                    acc[c0 + c + 2] = fmaf(x[c + 2], f.z * ws, acc[c0 + c + 2]);
-                    acc[c0 + c + 3] = fmaf(x[c + 3], f.w * ws, acc[c0 + c + 3]);
+                    const float4 f = *reinterpret_cast<const float4 *>(sc + col0 + c0 + c);
+                    float2 &a0 = acc[(c0 + c) / 2], &a1 = acc[(c0 + c) / 2 + 1];
+                    a0 = ffma2(make_float2(x[c], x[c + 1]), fmul2(make_float2(f.x, f.y), ws), a0);
+                    a1 = ffma2(make_float2(x[c + 2], x[c + 3]), fmul2(make_float2(f.z, f.w), ws), a1);
                 }
             }
             tc_fence_before();
@@ -220,8 +234,8 @@ few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUte
     if (p.splits == 1) {
         if (warp >= 2 && all_ok && row < p.rows) {
 #pragma unroll
-            for (int t = 0; t < NT; ++t)
-                if (t < live) p.out[(size_t)(t0 + t) * p.rows + row] = acc[t];
+            for (int t = 0; t < L::COLS; ++t)
+                if (col0 + t < live) p.out[(size_t)(t0 + col0 + t) * p.rows + row] = t & 1 ? acc[t / 2].y : acc[t / 2].x;
         }
         return;
     }
@@ -232,17 +246,35 @@ few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUte
     int *good = reinterpret_cast<int *>(slots);               // this CTA's partial sums are complete
     if (warp >= 2) {
 #pragma unroll
-        for (int t = 0; t < NT; ++t) part[t * ROWS + lrow] = acc[t];
+        for (int t = 0; t < L::COLS; ++t) part[(col0 + t) * ROWS + lrow] = t & 1 ? acc[t / 2].y : acc[t / 2].x;
     }
     if (threadIdx.x == 0) *good = all_ok;
     cluster_sync();
-    if (warp >= 2 && row < p.rows) {
+    if (warp >= 2) {
         bool fine = true;
         for (int q = 0; q < p.splits; ++q) fine = fine && __float_as_int(ld_cluster_f32(cluster_map(good, q))) != 0;
-        for (int t = split; fine && t < live; t += p.splits) {
-            float v = 0.f;
-            for (int q = 0; q < p.splits; ++q) v += ld_cluster_f32(cluster_map(part + t * ROWS + lrow, q));
-            p.out[(size_t)(t0 + t) * p.rows + row] = v;
+        // a warp adds one token's 128 rows at a time, four rows a lane
+        const int row4 = rtile * ROWS + 4 * lane;
+        const bool vec = p.rows % 4 == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15) == 0;
+        const uint32_t mine = smem_addr(part) + 16 * lane;
+        for (int t = split + p.splits * (warp - 2); fine && t < live; t += p.splits * L::SUM_WARPS) {
+            float4 v[8];
+#pragma unroll
+            for (int q = 0; q < 8; ++q)
+                if (q < p.splits) v[q] = ld_cluster_f32x4(cluster_rank(mine + t * ROWS * 4, q));
+            float4 sum = v[0];
+#pragma unroll
+            for (int q = 1; q < 8; ++q)
+                if (q < p.splits) { sum.x += v[q].x; sum.y += v[q].y; sum.z += v[q].z; sum.w += v[q].w; }
+            float *dst = p.out + (size_t)(t0 + t) * p.rows + row4;
+            if (vec) {
+                if (row4 < p.rows) *reinterpret_cast<float4 *>(dst) = sum;
+            } else {
+                if (row4 < p.rows) dst[0] = sum.x;
+                if (row4 + 1 < p.rows) dst[1] = sum.y;
+                if (row4 + 2 < p.rows) dst[2] = sum.z;
+                if (row4 + 3 < p.rows) dst[3] = sum.w;
+            }
         }
     }
     cluster_sync();
@@ -334,26 +366,26 @@ many_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUt
                 while (!mbar_try_wait(full + q % L::STAGES, (q / L::STAGES) & 1) && clock64() - start < WAIT_LIMIT_CYCLES) {}
         }
     } else if (warp == 1) {
-        if (lane == 0) {
-            constexpr uint32_t idesc = idesc_e4m3(L::MT, L::NT);
-            const int n = mine * p.blocks;
-            for (int j = 0; j < n; ++j) {
-                const int s = j % L::STAGES, d = j % L::BUFS;
-                if (!mbar_wait(full + s, (j / L::STAGES) & 1, abort_flag)) break;
-                if (j >= L::BUFS && !mbar_wait(d_empty + d, (j / L::BUFS - 1) & 1, abort_flag)) break;
-                tc_fence_after();
-                const uint32_t x = smem_addr(smem + s * L::STAGE), w = x + L::X_BYTES;
+        constexpr uint32_t idesc = idesc_e4m3(L::MT, L::NT);
+        const uint32_t lead = elect_lane(), tm = __shfl_sync(0xffffffffu, tmem, 0);
+        const int n = mine * p.blocks;
+        for (int j = 0, s = 0, lap = 0; j < n; ++j) {
+            const int d = j & 1;
+            if (!warp_wait8(full + s, lap & 1, abort_flag)) break;
+            if (j >= 2 && !warp_wait8(d_empty + d, ((j >> 1) - 1) & 1, abort_flag)) break;
+            tc_fence_after();
+            const uint64_t x = sw128_desc(smem_addr(smem + s * L::STAGE), 16, 1024);
+            const uint64_t w = sw128_desc(smem_addr(smem + s * L::STAGE + L::X_BYTES), 16, 1024);
 #pragma unroll
-                for (int k = 0; k < KB / 32; ++k)
-                    mma_e4m3_ss(tmem + d * L::NT, sw128_desc(x + k * 32, 16, 1024), sw128_desc(w + k * 32, 16, 1024), idesc,
-                                k > 0 ? 1u : 0u);
-                mma_commit(empty + s);
-                mma_commit(d_full + d);
-            }
-            mma_commit(mma_done);
-            const long long start = clock64();
-            while (!mbar_try_wait(mma_done, 0) && clock64() - start < WAIT_LIMIT_CYCLES) {}
+            for (int k = 0; k < KB / 32; ++k)
+                mma_e4m3_ss_by(lead, tm + d * L::NT, x + 2 * k, w + 2 * k, idesc, k > 0 ? 1u : 0u);
+            mma_commit_by(lead, empty + s);
+            mma_commit_by(lead, d_full + d);
+            if (++s == L::STAGES) { s = 0; ++lap; }
         }
+        mma_commit_by(lead, mma_done);
+        const long long start = clock64();
+        while (!mbar_try_wait(mma_done, 0) && clock64() - start < WAIT_LIMIT_CYCLES) {}
     } else {
         // Warps 2-5 take the tile's columns [0, 128), warps 6-9 [128, 256);
         // thread = TMEM lane = token.
@@ -375,17 +407,18 @@ many_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUt
                 const float *sc = slots + slot * L::SLOT_FLOATS;
                 const float f = sc[lrow + lane] * sc[L::MT + half];
                 const float2 f2 = make_float2(f, f);
+                // 16 columns at a time, the next ones on their way during the arithmetic.
+                float x[2][16];
+                const uint32_t at = t_col + d * L::NT;
+                tmem_ld16(at, x[0]);
 #pragma unroll
-                for (int c0 = 0; c0 < 128; c0 += 32) {
-                    float x[2][16];
-                    tmem_ld16(t_col + d * L::NT + c0, x[0]);
-                    tmem_ld16(t_col + d * L::NT + c0 + 16, x[1]);
+                for (int c0 = 0; c0 < 128; c0 += 16) {
+                    const int now = c0 >> 4 & 1;
                     tmem_wait_ld();
+                    if (c0 < 112) tmem_ld16(at + c0 + 16, x[now ^ 1]);
 #pragma unroll
-                    for (int q = 0; q < 2; ++q)
-#pragma unroll
-                        for (int c = 0; c < 8; ++c)
-                            acc[c0 / 2 + q * 8 + c] = ffma2(make_float2(x[q][2 * c], x[q][2 * c + 1]), f2, acc[c0 / 2 + q * 8 + c]);
+                    for (int c = 0; c < 8; ++c)
+                        acc[c0 / 2 + c] = ffma2(make_float2(x[now][2 * c], x[now][2 * c + 1]), f2, acc[c0 / 2 + c]);
                 }
                 tc_fence_before();
                 __syncwarp();
@@ -454,14 +487,14 @@ template <int NT> void launch_few(Mm8Params p, const void *weights, const void *
     using L = Few<NT>;
     const int row_tiles = (p.rows + ROWS - 1) / ROWS, token_tiles = (p.tokens + NT - 1) / NT;
     // Split the width while the CTAs still fit the SMs at once and every CTA keeps four blocks or more.
-    const long long slots = 148LL * L::CTAS, tiles = (long long)row_tiles * token_tiles;
+    const long long slots = 148LL * 2, tiles = (long long)row_tiles * token_tiles;
     int splits = 1;
     while (splits < 8 && tiles * splits * 2 <= slots && p.blocks >= 8 * splits) splits *= 2;
     p.splits = splits;
     const CUtensorMap mw = codes_map(weights, width, p.rows, ROWS), mx = codes_map(x, width, p.tokens, NT);
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(splits, row_tiles, token_tiles);
-    cfg.blockDim = dim3(192);
+    cfg.blockDim = dim3(L::THREADS);
     cfg.dynamicSmemBytes = L::SMEM;
     cfg.stream = st;
     cudaLaunchAttribute attr[2];

@@ -15,6 +15,7 @@
 #include "common.cuh"
 #include "hotpath.h"
 
+#include <algorithm>
 #include <stdexcept>
 #include <string>
 
@@ -27,15 +28,33 @@ constexpr int CODES = BLK * HD8;                 // codes of one (block, head)
 __device__ __forceinline__ __half2 as_half2(uint32_t v) { return *reinterpret_cast<const __half2 *>(&v); }
 __device__ __forceinline__ uint32_t half2_word(__half2 h) { return *reinterpret_cast<const uint32_t *>(&h); }
 
-// x / s rounded to the nearest integer, ties to even, exactly: the product
-// with the approximate reciprocal is off by one at most, and the sign of
-// x - (q +- 1/2) s, which one fused multiply-add gives without error, says
-// which side of the border x lies on.
-__device__ __forceinline__ int nearest_code(float x, float s, float inv) {
-    const float q = rintf(x * inv);
-    const float above = fmaf(-(q + 0.5f), s, x), below = fmaf(-(q - 0.5f), s, x);
-    const int n = (int)q, odd = n & 1;
-    return n + ((above > 0.f || (above == 0.f && odd)) ? 1 : 0) - ((below < 0.f || (below == 0.f && odd)) ? 1 : 0);
+// Four codes: x / s rounded to the nearest integer, ties to even, exactly.
+// Adding 1.5 * 2^23 to x times the approximate reciprocal leaves the integer q
+// in the low bits, at most one off.  x - q s is exact: it is a multiple of the
+// last place of s and no larger than s (where the last place of x is finer, |x|
+// < s / 2 and q = 0).  So |x - q s| >= s / 2 tells the few q that may be
+// wrong, and its sign the side.
+__device__ __forceinline__ uint32_t nearest_codes(float4 x, float s, float inv) {
+    constexpr float magic = 12582912.f;
+    const float v[4] = {x.x, x.y, x.z, x.w}, half = 0.5f * s;
+    uint32_t t[4];
+    float far = 0.f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const float sum = fmaf(v[e], inv, magic);
+        t[e] = __float_as_uint(sum);
+        far = fmaxf(far, fabsf(fmaf(magic - sum, s, v[e])));
+    }
+    if (far >= half) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float rest = fmaf(magic - __uint_as_float(t[e]), s, v[e]);
+            const bool odd = t[e] & 1u;
+            if (rest > half || (rest == half && odd)) ++t[e];
+            else if (rest < -half || (rest == -half && odd)) --t[e];
+        }
+    }
+    return __byte_perm(__byte_perm(t[0], t[1], 0x0040), __byte_perm(t[2], t[3], 0x0040), 0x5410);
 }
 
 struct Cache8Side {
@@ -88,14 +107,10 @@ __global__ void __launch_bounds__(256) cache8_pack_kernel(const Cache8Params p) 
     for (int i = 0; i < 8; ++i) {
         uint32_t out[2] = {0u, 0u};
         if (live) {
-            const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float2 f = __half22float2(as_half2(w[e]));
-                const uint32_t a = (uint32_t)nearest_code(f.x, scale, inv) & 0xFFu;
-                const uint32_t b = (uint32_t)nearest_code(f.y, scale, inv) & 0xFFu;
-                out[e >> 1] |= (a | b << 8) << (16 * (e & 1));
-            }
+            const float2 a = __half22float2(as_half2(x[i].x)), b = __half22float2(as_half2(x[i].y));
+            const float2 c = __half22float2(as_half2(x[i].z)), d = __half22float2(as_half2(x[i].w));
+            out[0] = nearest_codes(make_float4(a.x, a.y, b.x, b.y), scale, inv);
+            out[1] = nearest_codes(make_float4(c.x, c.y, d.x, d.y), scale, inv);
         }
         *reinterpret_cast<uint2 *>(dst + (size_t)(warp + 8 * i) * HD8) = make_uint2(out[0], out[1]);
     }
@@ -127,10 +142,13 @@ __global__ void __launch_bounds__(256) cache8_unpack_kernel(const Cache8Params p
         uint32_t h[8];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const float a = (float)(int8_t)(w[e] & 0xFFu), b = (float)(int8_t)(w[e] >> 8 & 0xFFu);
-            const float d = (float)(int8_t)(w[e] >> 16 & 0xFFu), f = (float)(int8_t)(w[e] >> 24);
-            h[2 * e] = half2_word(__floats2half2_rn(a * scale, b * scale));
-            h[2 * e + 1] = half2_word(__floats2half2_rn(d * scale, f * scale));
+            // the byte code + 128 as the last byte of 2^23 + it; subtracting leaves the code
+            const uint32_t u = w[e] ^ 0x80808080u;
+            float f[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) f[k] = (__uint_as_float(__byte_perm(u, 0x4B000000u, 0x7540 + k)) - 8388736.f) * scale;
+            h[2 * e] = half2_word(__floats2half2_rn(f[0], f[1]));
+            h[2 * e + 1] = half2_word(__floats2half2_rn(f[2], f[3]));
         }
         uint4 *dst = reinterpret_cast<uint4 *>(side.rows + ((size_t)(r - p.begin) * KV + head) * HD8 + col);
         dst[0] = make_uint4(h[0], h[1], h[2], h[3]);
@@ -155,12 +173,68 @@ __device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
     return (uint32_t)lo | (uint32_t)hi << 16;
 }
 
-// One CTA per row.  A warp takes every (warps)-th block of 128 columns, lane l
-// the columns [4 l, 4 l + 4) of it, up to PER_WARP blocks in registers, so the
-// row is read once, its sum of squares meets in shared memory, and a block's
-// maximum is a reduction inside one warp.  VEC: rows are 16-byte aligned.
+// Columns [c, c + 4) of a row, zero past its end.  VEC: rows are 16-byte aligned.
+template <bool VEC> __device__ __forceinline__ void load_columns(const float *src, int c, int width, float (&d)[4]) {
+    if (VEC) {
+        const float4 f = c < width ? *reinterpret_cast<const float4 *>(src + c) : make_float4(0.f, 0.f, 0.f, 0.f);
+        d[0] = f.x; d[1] = f.y; d[2] = f.z; d[3] = f.w;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) d[e] = c + e < width ? src[c + e] : 0.f;
+    }
+}
+template <bool VEC> __device__ __forceinline__ void store_columns(float *dst, int c, int width, const float (&d)[4]) {
+    if (VEC) {
+        if (c < width) *reinterpret_cast<float4 *>(dst + c) = make_float4(d[0], d[1], d[2], d[3]);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (c + e < width) dst[c + e] = d[e];
+    }
+}
+// Scale and codes of one block of 128 columns, spread over a warp, lane l with [4 l, 4 l + 4).
+template <bool VEC>
+__device__ __forceinline__ void store_codes(const Norm8Params &p, int token, int block, int lane, const float (&v)[4]) {
+    // The magnitudes' bits order like the values, infinity and NaN above all others.
+    const uint32_t own = max(max(__float_as_uint(v[0]) & 0x7FFFFFFFu, __float_as_uint(v[1]) & 0x7FFFFFFFu),
+                             max(__float_as_uint(v[2]) & 0x7FFFFFFFu, __float_as_uint(v[3]) & 0x7FFFFFFFu));
+    const uint32_t bits = __reduce_max_sync(0xffffffffu, own);
+    const bool finite = bits < 0x7F800000u;
+    const float scale = finite ? __fdiv_rn(__uint_as_float(bits), 448.f) : __int_as_float(0x7FC00000);
+    if (lane == 0) p.scales[(size_t)block * p.tokens + token] = scale;
+    uint32_t codes = 0u;
+    if (finite && scale > 0.f) {
+        float q[4];
+        if (scale > 0x1p-100f) {
+            // the quotient from the reciprocal, with one correction by its remainder
+            const float inv = __frcp_rn(scale);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float near = v[e] * inv;
+                q[e] = fmaf(fmaf(-near, scale, v[e]), inv, near);
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) q[e] = __fdiv_rn(v[e], scale);
+        }
+        codes = e4m3x4(q[0], q[1], q[2], q[3]);
+    }
+    const int c = block * 128 + 4 * lane;
+    uint8_t *dst = p.codes + (size_t)token * p.width + c;
+    if (VEC) {
+        if (c < p.width) *reinterpret_cast<uint32_t *>(dst) = codes;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (c + e < p.width) dst[e] = (uint8_t)(codes >> (8 * e));
+    }
+}
+
+// One CTA per row.  A warp takes every (warps)-th block of 128 columns, up to
+// PER_WARP of them in registers, so the row is read once, its sum of squares
+// meets in shared memory, and a block's maximum is a reduction inside one warp.
 constexpr int PER_WARP = 5, MAX_WARPS = 28;   // 140 blocks: 17,920 columns
-template <bool NORM, bool VEC>
+template <bool VEC>
 __global__ void __launch_bounds__(32 * MAX_WARPS) norm8_kernel(const Norm8Params p) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
     const int token = blockIdx.x;
@@ -168,80 +242,56 @@ __global__ void __launch_bounds__(32 * MAX_WARPS) norm8_kernel(const Norm8Params
     __shared__ float red[32];
     grid_dependency_wait();
     if (threadIdx.x == 0) launch_dependents();
-    float v[PER_WARP][4];
-    auto load = [&](const float *src, int c, float (&d)[4]) {
-        if (VEC) {
-            const float4 f = c < p.width ? *reinterpret_cast<const float4 *>(src + c) : make_float4(0.f, 0.f, 0.f, 0.f);
-            d[0] = f.x; d[1] = f.y; d[2] = f.z; d[3] = f.w;
-        } else {
+    float v[PER_WARP][4], w[PER_WARP][4], ss[PER_WARP];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) d[e] = c + e < p.width ? src[c + e] : 0.f;
-        }
-    };
-    auto store = [&](float *dst, int c, const float (&d)[4]) {
-        if (VEC) {
-            if (c < p.width) *reinterpret_cast<float4 *>(dst + c) = make_float4(d[0], d[1], d[2], d[3]);
-        } else {
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (c + e < p.width) dst[c + e] = d[e];
-        }
-    };
-#pragma unroll
-    for (int i = 0; i < PER_WARP; ++i) load(p.x + row, (warp + i * warps) * 128 + 4 * lane, v[i]);
-    if (NORM) {
-        if (p.residual) {
-            float r[PER_WARP][4];
-#pragma unroll
-            for (int i = 0; i < PER_WARP; ++i) load(p.residual + row, (warp + i * warps) * 128 + 4 * lane, r[i]);
-#pragma unroll
-            for (int i = 0; i < PER_WARP; ++i)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) v[i][e] += r[i][e];
-        }
-        float w[PER_WARP][4], ss[PER_WARP];
-#pragma unroll
-        for (int i = 0; i < PER_WARP; ++i) load(p.weights, (warp + i * warps) * 128 + 4 * lane, w[i]);
+    for (int i = 0; i < PER_WARP; ++i) load_columns<VEC>(p.x + row, (warp + i * warps) * 128 + 4 * lane, p.width, v[i]);
+    if (p.residual) {
+        float r[PER_WARP][4];
 #pragma unroll
         for (int i = 0; i < PER_WARP; ++i)
-            ss[i] = (v[i][0] * v[i][0] + v[i][1] * v[i][1]) + (v[i][2] * v[i][2] + v[i][3] * v[i][3]);
-        const float s = warp_sum((ss[0] + ss[1]) + (ss[2] + ss[3]) + ss[4]);
-        if (lane == 0) red[warp] = s;
-        __syncthreads();
-        const float all = warp_sum(lane < warps ? red[lane] : 0.f);
-        const float inv = __frsqrt_rn(__fdiv_rn(all, (float)p.width) + p.eps);
+            load_columns<VEC>(p.residual + row, (warp + i * warps) * 128 + 4 * lane, p.width, r[i]);
 #pragma unroll
-        for (int i = 0; i < PER_WARP; ++i) {
-            const int c = (warp + i * warps) * 128 + 4 * lane;
-            if (p.sum_out) store(p.sum_out + row, c, v[i]);
+        for (int i = 0; i < PER_WARP; ++i)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[i][e] = v[i][e] * inv * w[i][e];
-            if (p.normed) store(p.normed + row, c, v[i]);
-        }
+            for (int e = 0; e < 4; ++e) v[i][e] += r[i][e];
     }
+#pragma unroll
+    for (int i = 0; i < PER_WARP; ++i) load_columns<VEC>(p.weights, (warp + i * warps) * 128 + 4 * lane, p.width, w[i]);
+#pragma unroll
+    for (int i = 0; i < PER_WARP; ++i)
+        ss[i] = (v[i][0] * v[i][0] + v[i][1] * v[i][1]) + (v[i][2] * v[i][2] + v[i][3] * v[i][3]);
+    const float s = warp_sum((ss[0] + ss[1]) + (ss[2] + ss[3]) + ss[4]);
+    if (lane == 0) red[warp] = s;
+    __syncthreads();
+    const float all = warp_sum(lane < warps ? red[lane] : 0.f);
+    const float inv = __frsqrt_rn(__fdiv_rn(all, (float)p.width) + p.eps);
 #pragma unroll
     for (int i = 0; i < PER_WARP; ++i) {
         const int block = warp + i * warps, c = block * 128 + 4 * lane;
-        if (block >= p.blocks) continue;                       // the same for the whole warp
-        // The magnitudes' bits order like the values, infinity and NaN above all others.
-        const uint32_t own = max(max(__float_as_uint(v[i][0]) & 0x7FFFFFFFu, __float_as_uint(v[i][1]) & 0x7FFFFFFFu),
-                                 max(__float_as_uint(v[i][2]) & 0x7FFFFFFFu, __float_as_uint(v[i][3]) & 0x7FFFFFFFu));
-        const uint32_t bits = __reduce_max_sync(0xffffffffu, own);
-        const bool finite = bits < 0x7F800000u;
-        const float scale = finite ? __fdiv_rn(__uint_as_float(bits), 448.f) : __int_as_float(0x7FC00000);
-        if (lane == 0) p.scales[(size_t)block * p.tokens + token] = scale;
-        uint32_t codes = 0u;
-        if (finite && scale > 0.f)
-            codes = e4m3x4(__fdiv_rn(v[i][0], scale), __fdiv_rn(v[i][1], scale), __fdiv_rn(v[i][2], scale),
-                           __fdiv_rn(v[i][3], scale));
-        if (VEC) {
-            if (c < p.width) *reinterpret_cast<uint32_t *>(p.codes + row + c) = codes;
-        } else {
+        if (p.sum_out) store_columns<VEC>(p.sum_out + row, c, p.width, v[i]);
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (c + e < p.width) p.codes[row + c + e] = (uint8_t)(codes >> (8 * e));
-        }
+        for (int e = 0; e < 4; ++e) v[i][e] = v[i][e] * inv * w[i][e];
+        if (p.normed) store_columns<VEC>(p.normed + row, c, p.width, v[i]);
+        if (block < p.blocks) store_codes<VEC>(p, token, block, lane, v[i]);
     }
+}
+
+// The codes alone: every warp takes QUANT_BLOCKS blocks of 128 columns of a row,
+// independent of all others.
+constexpr int QUANT_BLOCKS = 4;
+template <bool VEC>
+__global__ void __launch_bounds__(256) quantize8_kernel(const Norm8Params p) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, token = blockIdx.x;
+    const int block0 = (blockIdx.y * 8 + warp) * QUANT_BLOCKS;
+    const size_t row = (size_t)token * p.width;
+    grid_dependency_wait();
+    if (threadIdx.x == 0) launch_dependents();
+    float v[QUANT_BLOCKS][4];
+#pragma unroll
+    for (int i = 0; i < QUANT_BLOCKS; ++i) load_columns<VEC>(p.x + row, (block0 + i) * 128 + 4 * lane, p.width, v[i]);
+#pragma unroll
+    for (int i = 0; i < QUANT_BLOCKS; ++i)
+        if (block0 + i < p.blocks) store_codes<VEC>(p, token, block0 + i, lane, v[i]);
 }
 
 void launched(cudaError_t e, const char *what) {
@@ -272,12 +322,16 @@ void norm8(uint8_t *codes, float *scales, float *sum_out, float *normed, const f
     Norm8Params p{codes, scales, sum_out, normed, x, residual, weights, tokens, width, (width + 127) / 128, eps};
     const bool vec = width % 4 == 0 && aligned(codes, 4) && aligned(x, 16) && aligned(residual, 16) && aligned(weights, 16) &&
                      aligned(sum_out, 16) && aligned(normed, 16);
+    if (!weights) {
+        const dim3 grid(tokens, (p.blocks + 8 * QUANT_BLOCKS - 1) / (8 * QUANT_BLOCKS));
+        const int warps = std::min(8, (p.blocks + QUANT_BLOCKS - 1) / QUANT_BLOCKS);
+        launched(launch_chained(vec ? quantize8_kernel<true> : quantize8_kernel<false>, grid, dim3(32 * warps), 0, st, p), "quantize8");
+        return;
+    }
     // warps that hold the row in registers: PER_WARP blocks of 128 columns each
-    int warps = (p.blocks + PER_WARP - 1) / PER_WARP;
+    const int warps = (p.blocks + PER_WARP - 1) / PER_WARP;
     if (warps > MAX_WARPS) throw std::invalid_argument("the row is wider than a block of threads holds");
-    auto kernel = weights ? (vec ? norm8_kernel<true, true> : norm8_kernel<true, false>)
-                          : (vec ? norm8_kernel<false, true> : norm8_kernel<false, false>);
-    launched(launch_chained(kernel, dim3(tokens), dim3(32 * warps), 0, st, p), weights ? "norm8" : "quantize8");
+    launched(launch_chained(vec ? norm8_kernel<true> : norm8_kernel<false>, dim3(tokens), dim3(32 * warps), 0, st, p), "norm8");
 }
 
 }  // namespace qv

@@ -104,11 +104,12 @@ class NativeError(RuntimeError):
 
 
 # Host-side checks of the 8-bit calls, which take their sizes from the tensors: a wrong shape, element
-# size, layout or device is refused here, before an address reaches a kernel.
+# size, layout or device is refused here, before an address reaches a kernel.  They run on every call of
+# a decode step, so they ask a tensor only what is cheap to ask (a CPU tensor's device number is -1).
 def need_tensor(t, itemsize, shape, name, device):
-    if t.element_size() != itemsize or t.shape != shape or not t.is_contiguous() or not t.is_cuda or t.device != device:
-        raise ValueError(f'{name} must be a contiguous CUDA tensor of shape {list(shape)} with {itemsize}-byte elements '
-                         f'on {device}')
+    if t.shape != shape or t.element_size() != itemsize or t.get_device() != device or device < 0 or not t.is_contiguous():
+        raise ValueError(f'{name} must be a contiguous CUDA tensor of shape {list(shape)} with {itemsize}-byte elements'
+                         + (f' on device {device}' if device >= 0 else ''))
 
 
 def need_cache8(key_codes, key_scales, value_codes, value_scales, end, device):
@@ -273,21 +274,22 @@ class HotPath:
 
     # -- 8-bit serving ------------------------------------------------------
     def _call(self, device, function, *args):
-        """function(*args, stream) with the tensors' device current, on torch's current stream of it."""
+        """function(*args, stream) with device number `device` current, on torch's current stream of it."""
         import torch
-        stream = torch.cuda.current_stream(device).cuda_stream
-        if torch.cuda.current_device() == device.index:
+        stream = torch._C._cuda_getCurrentRawStream(device)      # what torch.cuda.current_stream(device) wraps
+        if torch._C._cuda_getDevice() == device:
             code = function(*args, stream)
         else:
             with torch.cuda.device(device):
                 code = function(*args, stream)
-        self.check(code)
+        if code:
+            self.check(code)
 
     def norm8(self, codes, scales, x, weights, residual=None, residual_out=None, normed=None, epsilon=1e-6):
         """qv_norm8: e4m3 codes [tokens][width] and scales [ceil(width/128)][tokens] of the RMSNorm of
         x (+ residual); residual_out and normed, where given, receive the sum and the norm in fp32."""
         tokens, width = x.shape
-        dev = x.device
+        dev = x.get_device()
         need_tensor(x, 4, (tokens, width), 'x', dev)
         need_tensor(codes, 1, (tokens, width), 'codes', dev)
         need_tensor(scales, 4, (-(-width // 128), tokens), 'scales', dev)
@@ -303,7 +305,7 @@ class HotPath:
     def quantize8(self, codes, scales, x):
         """qv_quantize8: e4m3 codes and scales of x itself."""
         tokens, width = x.shape
-        dev = x.device
+        dev = x.get_device()
         need_tensor(x, 4, (tokens, width), 'x', dev)
         need_tensor(codes, 1, (tokens, width), 'codes', dev)
         need_tensor(scales, 4, (-(-width // 128), tokens), 'scales', dev)
@@ -312,7 +314,7 @@ class HotPath:
     def mm8(self, out, weights, weight_scales, codes, scales):
         """qv_mm8: out [tokens][rows] = codes x weights^T, both e4m3 with a scale for every block of 128."""
         tokens, width = codes.shape
-        rows, blocks, dev = weights.shape[0], -(-width // 128), codes.device
+        rows, blocks, dev = weights.shape[0], -(-width // 128), codes.get_device()
         need_tensor(codes, 1, (tokens, width), 'codes', dev)
         need_tensor(scales, 4, (blocks, tokens), 'scales', dev)
         need_tensor(weights, 1, (rows, width), 'weights', dev)
@@ -337,7 +339,7 @@ class HotPath:
         positions and the fp16 tail.  Without `workspace`, one that is kept for the current stream is used;
         under graph capture it has to be given (attention8_workspace), since the graph goes on using it."""
         import torch
-        dev, tail = out.device, key_tail.shape[0]
+        dev, tail = out.get_device(), key_tail.shape[0]
         need_tensor(out, 4, (batch, 24, 256), 'out', dev)
         need_tensor(q_gate, 4, (batch, 24, 512), 'q_gate', dev)
         need_tensor(key, 4, (batch, 4, 256), 'key', dev)
@@ -350,10 +352,10 @@ class HotPath:
         if workspace is None:
             if torch.cuda.is_current_stream_capturing():
                 raise ValueError('attention8 under graph capture needs a workspace of its own (attention8_workspace)')
-            which = (dev.index, torch.cuda.current_stream(dev).cuda_stream)
+            which = (dev, torch._C._cuda_getCurrentRawStream(dev))
             workspace = self._workspaces8.get(which)
             if workspace is None:
-                workspace = self._workspaces8[which] = self.attention8_workspace(dev)
+                workspace = self._workspaces8[which] = self.attention8_workspace(out.device)
         else:
             need_tensor(workspace, 1, workspace.shape, 'workspace', dev)
         self._call(dev, self.lib.qv_attention8, out.data_ptr(), key_codes.data_ptr(), key_scales.data_ptr(),
@@ -363,7 +365,7 @@ class HotPath:
 
     def cache8_pack(self, key_codes, key_scales, value_codes, value_scales, key_rows, value_rows, begin, end):
         """qv_cache8_pack: positions [begin, end) of fp16 rows (position r at row r % rows) to int8 codes."""
-        ring, dev = key_rows.shape[0], key_rows.device
+        ring, dev = key_rows.shape[0], key_rows.get_device()
         need_cache8(key_codes, key_scales, value_codes, value_scales, end, dev)
         need_tensor(key_rows, 2, (ring, 4, 256), 'key_rows', dev)
         need_tensor(value_rows, 2, (ring, 4, 256), 'value_rows', dev)
@@ -372,7 +374,7 @@ class HotPath:
 
     def cache8_unpack(self, key_rows, value_rows, key_codes, key_scales, value_codes, value_scales, begin, end, origin=0):
         """qv_cache8_unpack: positions [begin, end) as fp16 rows, position r at row r - origin."""
-        rows, dev = key_rows.shape[0], key_rows.device
+        rows, dev = key_rows.shape[0], key_rows.get_device()
         need_cache8(key_codes, key_scales, value_codes, value_scales, end, dev)
         need_tensor(key_rows, 2, (rows, 4, 256), 'key_rows', dev)
         need_tensor(value_rows, 2, (rows, 4, 256), 'value_rows', dev)
