@@ -14,9 +14,9 @@
 //    over a cluster of up to 8 CTAs whose partial sums meet in distributed
 //    shared memory in a fixed order, so that also few rows fill the SMs and no
 //    workspace or atomics are needed.
-//  * many_kernel (128 tokens as the MMA's M, 256 weight rows as its N):
-//    persistent CTAs.  Bound by the tensor pipe; with tokens in the TMEM lanes
-//    the two scales of a thread's columns are one factor per block.
+//  * many_kernel (128 tokens as the MMA's M, 256 weight rows as its N): persistent
+//    CTAs.  Bound by the tensor pipe; with tokens in the TMEM lanes the two scales
+//    of a thread's columns are one factor per block.
 #include "common.cuh"
 #include "hotpath.h"
 
@@ -86,12 +86,13 @@ struct Mm8Params {
 
 // ---------------------------------------------------------------- few tokens
 template <int NT> struct Few {
-    // Two CTAs per SM: their rings hold 2 x 96..108 KB in flight, enough for the
-    // HBM latency.  Four warps scale and add up to 32 tokens, eight beyond.
-    static constexpr int STAGES = NT == 16 ? 6 : NT == 32 ? 5 : NT == 64 ? 4 : 3;
+    // Two CTAs per SM up to 64 tokens, one at 128: their rings hold 192 KB or more
+    // in flight.  Four warps scale and add up to 32 tokens, eight beyond.
+    static constexpr int CTAS = NT <= 64 ? 2 : 1;
+    static constexpr int STAGES = NT == 16 ? 6 : NT == 32 ? 5 : NT == 64 ? 4 : 6;
     static constexpr int BUFS = NT <= 32 ? 4 : 2;            // TMEM accumulators
     static constexpr int SUM_WARPS = NT <= 32 ? 4 : 8, COLS = NT * 4 / SUM_WARPS;   // columns of a warp
-    static constexpr int THREADS = 64 + 32 * SUM_WARPS;
+    static constexpr int THREADS = 32 * (3 + SUM_WARPS), SCALE_WARP = 2 + SUM_WARPS;
     static constexpr int SLOTS = STAGES + BUFS;              // scale slots
     static constexpr int W_BYTES = ROWS * KB, X_BYTES = NT * KB, STAGE = W_BYTES + X_BYTES;
     static constexpr int SLOT_FLOATS = NT + 4;
@@ -103,7 +104,7 @@ template <int NT> struct Few {
 };
 
 template <int NT>
-__global__ void __launch_bounds__(Few<NT>::THREADS, 2)
+__global__ void __launch_bounds__(Few<NT>::THREADS, Few<NT>::CTAS)
 few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX, const Mm8Params p) {
     using L = Few<NT>;
     extern __shared__ __align__(1024) uint8_t smem[];
@@ -145,35 +146,54 @@ few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUte
     const int col0 = (warp - 2) / 4 * L::COLS;                 // this warp's tokens of the tile
     bool ok = !bad_base;
     if (warp == 0) {
-        // ------------------------------------------------ producer: code tiles by TMA, scales by small copies
+        // ------------------------------------------------ producer
+        const uint32_t lead = elect_lane();
         int issued = 0;
-        for (int j = 0; j < n && ok; ++j) {
-            const int s = j % L::STAGES, slot = j % L::SLOTS, b = b0 + j;
-            if (j >= L::STAGES && !warp_wait8(empty + s, (j / L::STAGES - 1) & 1, abort_flag)) { ok = false; break; }
-            if (lane == 0) {
+        for (int j = 0, s = 0, lap = 0; j < n; ++j) {
+            if (lap > 0 && !warp_wait8(empty + s, (lap - 1) & 1, abort_flag)) { ok = false; break; }
+            if (lead) {
                 uint8_t *w = smem + s * L::STAGE;
                 mbar_expect_tx(full + s, L::STAGE);
-                tma_load_2d(w, &tmW, full + s, b * KB, rtile * ROWS);
-                tma_load_2d(w + L::W_BYTES, &tmX, full + s, b * KB, t0);
+                tma_load_2d(w, &tmW, full + s, (b0 + j) * KB, rtile * ROWS);
+                tma_load_2d(w + L::W_BYTES, &tmX, full + s, (b0 + j) * KB, t0);
             }
+            __syncwarp();
             issued = j + 1;
-            // A slot is free again here: the MMA of block j - STAGES has run,
-            // which waited until block j - SLOTS had left its accumulator.
-            float *d = slots + slot * L::SLOT_FLOATS;
-            for (int t = lane; t < NT; t += 32) {
-                const bool live = t0 + t < p.tokens;
-                copy_float(d + t, p.scales + (size_t)b * p.tokens + (live ? t0 + t : 0), live);
-            }
-            if (lane == 0) copy_float(d + NT, p.weight_scales + (size_t)rtile * p.blocks + b, true);
-            arrive_copies(s_full + slot);
+            if (++s == L::STAGES) { s = 0; ++lap; }
         }
-        asm volatile("cp.async.wait_all;" ::: "memory");
         // Every issued load must land before the CTA may exit or reuse the ring.
-        if (lane == 0) {
+        if (lead) {
             const long long start = clock64();
             for (int j = max(0, issued - L::STAGES); j < issued; ++j)
                 while (!mbar_try_wait(full + j % L::STAGES, (j / L::STAGES) & 1) && clock64() - start < WAIT_LIMIT_CYCLES) {}
         }
+    } else if (warp == L::SCALE_WARP) {
+        // ------------------------------------------------ scales, by small copies
+        constexpr int PER_LANE = (NT + 31) / 32;
+        const float *src[PER_LANE], *w_src = p.weight_scales + (size_t)rtile * p.blocks + b0;
+        bool live[PER_LANE];
+#pragma unroll
+        for (int i = 0; i < PER_LANE; ++i) {
+            const int t = 32 * i + lane;
+            live[i] = t < NT && t0 + t < p.tokens;
+            src[i] = p.scales + (size_t)b0 * p.tokens + (live[i] ? t0 + t : 0);
+        }
+        for (int j = 0, s = 0, lap = 0, slot = 0; j < n; ++j) {
+            // A slot is free with its stage: the MMA of block j - STAGES has run,
+            // which waited until block j - SLOTS had left its accumulator.
+            if (lap > 0 && !warp_wait8(empty + s, (lap - 1) & 1, abort_flag)) { ok = false; break; }
+            float *d = slots + slot * L::SLOT_FLOATS;
+#pragma unroll
+            for (int i = 0; i < PER_LANE; ++i) {
+                if (32 * i + lane < NT) copy_float(d + 32 * i + lane, src[i], live[i]);
+                src[i] += p.tokens;
+            }
+            if (lane == 0) copy_float(d + NT, w_src + j, true);
+            arrive_copies(s_full + slot);
+            if (++s == L::STAGES) { s = 0; ++lap; }
+            if (++slot == L::SLOTS) slot = 0;
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
     } else if (warp == 1) {
         // ------------------------------------------------ MMA issuer
         constexpr uint32_t idesc = idesc_e4m3(ROWS, NT);
@@ -232,7 +252,7 @@ few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUte
     const int lrow = (warp & 3) * 32 + lane, row = rtile * ROWS + lrow;
     const int live = min(NT, p.tokens - t0);
     if (p.splits == 1) {
-        if (warp >= 2 && all_ok && row < p.rows) {
+        if (warp >= 2 && warp < L::SCALE_WARP && all_ok && row < p.rows) {
 #pragma unroll
             for (int t = 0; t < L::COLS; ++t)
                 if (col0 + t < live) p.out[(size_t)(t0 + col0 + t) * p.rows + row] = t & 1 ? acc[t / 2].y : acc[t / 2].x;
@@ -244,13 +264,14 @@ few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUte
     // splits.  Every CTA of the cluster passes both barriers.
     float *part = reinterpret_cast<float *>(smem);
     int *good = reinterpret_cast<int *>(slots);               // this CTA's partial sums are complete
-    if (warp >= 2) {
+    const bool sums = warp >= 2 && warp < L::SCALE_WARP;
+    if (sums) {
 #pragma unroll
         for (int t = 0; t < L::COLS; ++t) part[(col0 + t) * ROWS + lrow] = t & 1 ? acc[t / 2].y : acc[t / 2].x;
     }
     if (threadIdx.x == 0) *good = all_ok;
     cluster_sync();
-    if (warp >= 2) {
+    if (sums) {
         bool fine = true;
         for (int q = 0; q < p.splits; ++q) fine = fine && __float_as_int(ld_cluster_f32(cluster_map(good, q))) != 0;
         // a warp adds one token's 128 rows at a time, four rows a lane
@@ -281,35 +302,42 @@ few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUte
 }
 
 // ---------------------------------------------------------------- many tokens
+// TMEM holds two blocks' sums (2 x 256 columns), so a block takes half of its
+// way from the MMA through the scaling warps and back.  What shortens that way:
+// the weight rows' halves go it separately, sixteen warps empty a block (64 sums
+// a thread; four warps on each scheduler hide the loads' latency), the scales are
+// in registers before the sums are there, and nobody else does the issuing
+// warps' work (copies of scales have a warp of their own).
 struct Many {
     static constexpr int MT = 128, NT = 256;                 // tokens, weight rows of a tile
     static constexpr int STAGES = 4, BUFS = 2, SLOTS = STAGES + BUFS;
+    static constexpr int SUM_WARPS = 16, COLS = NT * 4 / SUM_WARPS, THREADS = 32 * (3 + SUM_WARPS), SCALE_WARP = 2 + SUM_WARPS;
     static constexpr int X_BYTES = MT * KB, W_BYTES = NT * KB, STAGE = X_BYTES + W_BYTES;
     static constexpr int SLOT_FLOATS = MT + 4;
-    static constexpr int OUT_ROW = 20;                       // floats of a staged row: 16 columns and a pad
-    static constexpr int SM_OUT = STAGES * STAGE;            // [8 warps][32 rows][OUT_ROW]
-    static constexpr int SM_SCALE = SM_OUT + 8 * 32 * OUT_ROW * 4;
+    static constexpr int OUT_ROW = 12;                       // floats of a staged row: 8 columns and a pad
+    static constexpr int SM_OUT = STAGES * STAGE;            // [SUM_WARPS][32 rows][OUT_ROW]
+    static constexpr int SM_SCALE = SM_OUT + SUM_WARPS * 32 * OUT_ROW * 4;
     static constexpr int SM_BAR = SM_SCALE + SLOTS * SLOT_FLOATS * 4;
     static constexpr int SMEM = SM_BAR + 256;
     static_assert(SMEM <= 227 * 1024, "shared memory of a CTA");
 };
 
-__global__ void __launch_bounds__(320, 1)
+__global__ void __launch_bounds__(Many::THREADS, 1)
 many_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX, const Mm8Params p) {
     using L = Many;
     extern __shared__ __align__(1024) uint8_t smem[];
     uint64_t *full = reinterpret_cast<uint64_t *>(smem + L::SM_BAR), *empty = full + L::STAGES;
-    uint64_t *d_full = empty + L::STAGES, *d_empty = d_full + L::BUFS, *s_full = d_empty + L::BUFS;
+    uint64_t *d_full = empty + L::STAGES, *d_empty = d_full + 2 * L::BUFS, *s_full = d_empty + 2 * L::BUFS;   // d: [buffer][half]
     uint64_t *mma_done = s_full + L::SLOTS;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(mma_done + 1);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
     float *slots = reinterpret_cast<float *>(smem + L::SM_SCALE);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const bool bad_base = (smem_addr(smem) & 1023) != 0;
+    const bool bad_base = (smem_addr(smem) & 1023) != 0;      // 128B-swizzle atoms need a 1024-byte aligned base
     if (threadIdx.x == 0) {
         for (int i = 0; i < L::STAGES; ++i) { mbar_init(full + i, 1); mbar_init(empty + i, 1); }
-        for (int i = 0; i < L::BUFS; ++i) { mbar_init(d_full + i, 1); mbar_init(d_empty + i, 8); }
+        for (int i = 0; i < 2 * L::BUFS; ++i) { mbar_init(d_full + i, 1); mbar_init(d_empty + i, L::SUM_WARPS / 2); }
         for (int i = 0; i < L::SLOTS; ++i) mbar_init(s_full + i, 32);
         mbar_init(mma_done, 1);
         *abort_flag = bad_base ? 1 : 0;
@@ -332,114 +360,143 @@ many_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUt
     const int row_blocks = (p.rows + ROWS - 1) / ROWS;
     if (bad_base) {
     } else if (warp == 0) {
-        int j = 0;                                           // blocks since the start, over all tiles
+        // ------------------------------------------------ producer
+        const uint32_t lead = elect_lane();
+        int j = 0, s = 0, lap = 0;                           // j: blocks since the start, over all tiles
         bool ok = true;
         for (int i = 0; i < mine && ok; ++i) {
             const int tile = blockIdx.x + i * gridDim.x, m0 = tile % p.m_tiles * L::MT, n0 = tile / p.m_tiles * L::NT;
             for (int b = 0; b < p.blocks; ++b, ++j) {
-                const int s = j % L::STAGES, slot = j % L::SLOTS;
-                if (j >= L::STAGES && !warp_wait8(empty + s, (j / L::STAGES - 1) & 1, abort_flag)) { ok = false; break; }
-                if (lane == 0) {
+                if (lap > 0 && !warp_wait8(empty + s, (lap - 1) & 1, abort_flag)) { ok = false; break; }
+                if (lead) {
                     uint8_t *x = smem + s * L::STAGE;
                     mbar_expect_tx(full + s, L::STAGE);
                     tma_load_2d(x, &tmX, full + s, b * KB, m0);
                     tma_load_2d(x + L::X_BYTES, &tmW, full + s, b * KB, n0);
                 }
-                float *d = slots + slot * L::SLOT_FLOATS;
-#pragma unroll
-                for (int t = 0; t < L::MT; t += 32) {
-                    const bool live = m0 + t + lane < p.tokens;
-                    copy_float(d + t + lane, p.scales + (size_t)b * p.tokens + (live ? m0 + t + lane : 0), live);
-                }
-                if (lane < 2) {
-                    const int rb = n0 / ROWS + lane;
-                    const bool live = rb < row_blocks;
-                    copy_float(d + L::MT + lane, p.weight_scales + (size_t)(live ? rb : 0) * p.blocks + b, live);
-                }
-                arrive_copies(s_full + slot);
+                __syncwarp();
+                if (++s == L::STAGES) { s = 0; ++lap; }
             }
         }
-        asm volatile("cp.async.wait_all;" ::: "memory");
-        if (lane == 0) {
+        // Every issued load must land before the CTA may exit.
+        if (lead) {
             const long long start = clock64();
             for (int q = max(0, j - L::STAGES); q < j; ++q)
                 while (!mbar_try_wait(full + q % L::STAGES, (q / L::STAGES) & 1) && clock64() - start < WAIT_LIMIT_CYCLES) {}
         }
     } else if (warp == 1) {
-        constexpr uint32_t idesc = idesc_e4m3(L::MT, L::NT);
+        // ------------------------------------------------ MMA issuer
+        constexpr uint32_t idesc = idesc_e4m3(L::MT, L::NT / 2);
         const uint32_t lead = elect_lane(), tm = __shfl_sync(0xffffffffu, tmem, 0);
         const int n = mine * p.blocks;
         for (int j = 0, s = 0, lap = 0; j < n; ++j) {
             const int d = j & 1;
             if (!warp_wait8(full + s, lap & 1, abort_flag)) break;
-            if (j >= 2 && !warp_wait8(d_empty + d, ((j >> 1) - 1) & 1, abort_flag)) break;
-            tc_fence_after();
             const uint64_t x = sw128_desc(smem_addr(smem + s * L::STAGE), 16, 1024);
             const uint64_t w = sw128_desc(smem_addr(smem + s * L::STAGE + L::X_BYTES), 16, 1024);
+            bool ok = true;
+            for (int h = 0; h < 2; ++h) {
+                ok = j < 2 || warp_wait8(d_empty + 2 * d + h, ((j >> 1) - 1) & 1, abort_flag);
+                if (!ok) break;
+                tc_fence_after();
 #pragma unroll
-            for (int k = 0; k < KB / 32; ++k)
-                mma_e4m3_ss_by(lead, tm + d * L::NT, x + 2 * k, w + 2 * k, idesc, k > 0 ? 1u : 0u);
+                for (int k = 0; k < KB / 32; ++k)
+                    mma_e4m3_ss_by(lead, tm + d * L::NT + h * (L::NT / 2), x + 2 * k, w + h * (L::W_BYTES / 32) + 2 * k, idesc,
+                                   k > 0 ? 1u : 0u);
+                mma_commit_by(lead, d_full + 2 * d + h);
+            }
+            if (!ok) break;
             mma_commit_by(lead, empty + s);
-            mma_commit_by(lead, d_full + d);
             if (++s == L::STAGES) { s = 0; ++lap; }
         }
         mma_commit_by(lead, mma_done);
         const long long start = clock64();
         while (!mbar_try_wait(mma_done, 0) && clock64() - start < WAIT_LIMIT_CYCLES) {}
-    } else {
-        // Warps 2-5 take the tile's columns [0, 128), warps 6-9 [128, 256);
-        // thread = TMEM lane = token.
-        const int half = (warp - 2) >> 2, lrow = (warp & 3) * 32;
-        const uint32_t t_col = tmem + ((uint32_t)lrow << 16) + half * 128;
-        float *stage = reinterpret_cast<float *>(smem + L::SM_OUT) + (warp - 2) * 32 * L::OUT_ROW;
-        int j = 0;
+    } else if (warp == L::SCALE_WARP) {
+        // ------------------------------------------------ scales, by small copies
+        int s = 0, lap = 0, slot = 0;
         bool ok = true;
         for (int i = 0; i < mine && ok; ++i) {
             const int tile = blockIdx.x + i * gridDim.x, m0 = tile % p.m_tiles * L::MT, n0 = tile / p.m_tiles * L::NT;
-            float2 acc[64];
+            bool live[4];
+            const float *src[4];
 #pragma unroll
-            for (int c = 0; c < 64; ++c) acc[c] = make_float2(0.f, 0.f);
+            for (int t = 0; t < 4; ++t) {
+                live[t] = m0 + 32 * t + lane < p.tokens;
+                src[t] = p.scales + (live[t] ? m0 + 32 * t + lane : 0);
+            }
+            const bool w_live = n0 / ROWS + lane < row_blocks;
+            const float *w_src = p.weight_scales + (size_t)(w_live ? n0 / ROWS + lane : 0) * p.blocks;
+            for (int b = 0; b < p.blocks; ++b) {
+                // A slot is free with its stage: the MMA of the block STAGES before has
+                // run, which waited until the block SLOTS before had left TMEM.
+                if (lap > 0 && !warp_wait8(empty + s, (lap - 1) & 1, abort_flag)) { ok = false; break; }
+                float *d = slots + slot * L::SLOT_FLOATS;
+#pragma unroll
+                for (int t = 0; t < 4; ++t) {
+                    copy_float(d + 32 * t + lane, src[t], live[t]);
+                    src[t] += p.tokens;
+                }
+                if (lane < 2) copy_float(d + L::MT + lane, w_src + b, w_live);
+                arrive_copies(s_full + slot);
+                if (++s == L::STAGES) { s = 0; ++lap; }
+                if (++slot == L::SLOTS) slot = 0;
+            }
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+    } else {
+        // ------------------------------------------------ sums
+        // Four warps a quarter of TMEM's lanes, 64 columns each; thread = lane = token.
+        const int group = (warp - 2) >> 2, half = group >> 1, lrow = (warp & 3) * 32;
+        const uint32_t t_col = tmem + ((uint32_t)lrow << 16) + group * L::COLS;
+        float *stage = reinterpret_cast<float *>(smem + L::SM_OUT) + (warp - 2) * 32 * L::OUT_ROW;
+        const bool vec = p.rows % 4 == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15) == 0;
+        int j = 0, slot = 0, slap = 0;
+        bool ok = true;
+        for (int i = 0; i < mine && ok; ++i) {
+            const int tile = blockIdx.x + i * gridDim.x, m0 = tile % p.m_tiles * L::MT, n0 = tile / p.m_tiles * L::NT;
+            float2 acc[L::COLS / 2];
+#pragma unroll
+            for (int c = 0; c < L::COLS / 2; ++c) acc[c] = make_float2(0.f, 0.f);
             for (int b = 0; b < p.blocks; ++b, ++j) {
-                const int d = j % L::BUFS, slot = j % L::SLOTS;
-                if (!warp_wait8(s_full + slot, (j / L::SLOTS) & 1, abort_flag) ||
-                    !warp_wait8(d_full + d, (j / L::BUFS) & 1, abort_flag)) { ok = false; break; }
-                tc_fence_after();
+                const int d = j & 1;
+                if (!warp_wait8(s_full + slot, slap & 1, abort_flag)) { ok = false; break; }
                 const float *sc = slots + slot * L::SLOT_FLOATS;
                 const float f = sc[lrow + lane] * sc[L::MT + half];
                 const float2 f2 = make_float2(f, f);
-                // 16 columns at a time, the next ones on their way during the arithmetic.
-                float x[2][16];
-                const uint32_t at = t_col + d * L::NT;
-                tmem_ld16(at, x[0]);
+                if (!warp_wait8(d_full + 2 * d + half, (j >> 1) & 1, abort_flag)) { ok = false; break; }
+                tc_fence_after();
 #pragma unroll
-                for (int c0 = 0; c0 < 128; c0 += 16) {
-                    const int now = c0 >> 4 & 1;
+                for (int c0 = 0; c0 < L::COLS; c0 += 16) {
+                    float x[16];
+                    tmem_ld16(t_col + d * L::NT + c0, x);
                     tmem_wait_ld();
-                    if (c0 < 112) tmem_ld16(at + c0 + 16, x[now ^ 1]);
+                    if (c0 + 16 == L::COLS) {
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(d_empty + 2 * d + half);
+                    }
 #pragma unroll
                     for (int c = 0; c < 8; ++c)
-                        acc[c0 / 2 + c] = ffma2(make_float2(x[now][2 * c], x[now][2 * c + 1]), f2, acc[c0 / 2 + c]);
+                        acc[c0 / 2 + c] = ffma2(make_float2(x[2 * c], x[2 * c + 1]), f2, acc[c0 / 2 + c]);
                 }
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(d_empty + d);
+                if (++slot == L::SLOTS) { slot = 0; ++slap; }
             }
             if (!ok) break;
-            // 16 columns at a time through shared memory: 64-byte pieces of eight rows per store.
-            const bool vec = p.rows % 4 == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15) == 0;
+            // 8 columns at a time through shared memory: whole 32-byte sectors of sixteen rows per store.
 #pragma unroll
-            for (int c0 = 0; c0 < 128; c0 += 16) {
+            for (int c0 = 0; c0 < L::COLS; c0 += 8) {
 #pragma unroll
-                for (int c = 0; c < 16; c += 4) {
+                for (int c = 0; c < 8; c += 4) {
                     const float2 a = acc[(c0 + c) / 2], e = acc[(c0 + c) / 2 + 1];
                     *reinterpret_cast<float4 *>(stage + lane * L::OUT_ROW + c) = make_float4(a.x, a.y, e.x, e.y);
                 }
                 __syncwarp();
-                const int col = n0 + half * 128 + c0 + (lane & 3) * 4;
+                const int col = n0 + group * L::COLS + c0 + (lane & 1) * 4;
 #pragma unroll
-                for (int r0 = 0; r0 < 32; r0 += 8) {
-                    const int r = r0 + (lane >> 2), token = m0 + lrow + r;
-                    const float4 v = *reinterpret_cast<const float4 *>(stage + r * L::OUT_ROW + (lane & 3) * 4);
+                for (int r0 = 0; r0 < 32; r0 += 16) {
+                    const int r = r0 + (lane >> 1), token = m0 + lrow + r;
+                    const float4 v = *reinterpret_cast<const float4 *>(stage + r * L::OUT_ROW + (lane & 1) * 4);
                     if (token >= p.tokens) continue;
                     float *dst = p.out + (size_t)token * p.rows + col;
                     if (vec) {
@@ -483,31 +540,37 @@ template <class K> void reserve(K *kernel, int bytes) {
         throw std::runtime_error("cannot reserve shared memory for the e4m3 product");
 }
 
-template <int NT> void launch_few(Mm8Params p, const void *weights, const void *x, int width, cudaStream_t st) {
-    using L = Few<NT>;
-    const int row_tiles = (p.rows + ROWS - 1) / ROWS, token_tiles = (p.tokens + NT - 1) / NT;
-    // Split the width while the CTAs still fit the SMs at once and every CTA keeps four blocks or more.
-    const long long slots = 148LL * 2, tiles = (long long)row_tiles * token_tiles;
-    int splits = 1;
-    while (splits < 8 && tiles * splits * 2 <= slots && p.blocks >= 8 * splits) splits *= 2;
-    p.splits = splits;
-    const CUtensorMap mw = codes_map(weights, width, p.rows, ROWS), mx = codes_map(x, width, p.tokens, NT);
+template <class K>
+void launch_cluster(K *kernel, dim3 grid, int threads, int smem, int cluster, cudaStream_t st, const CUtensorMap &mw,
+                    const CUtensorMap &mx, const Mm8Params &p) {
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(splits, row_tiles, token_tiles);
-    cfg.blockDim = dim3(L::THREADS);
-    cfg.dynamicSmemBytes = L::SMEM;
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = splits;
+    attr[1].val.clusterDim.x = cluster;
     attr[1].val.clusterDim.y = 1;
     attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, few_kernel<NT>, mw, mx, p);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, mw, mx, p);
     if (e != cudaSuccess) throw std::runtime_error(std::string("e4m3 product: ") + cudaGetErrorString(e));
+}
+
+template <int NT> void launch_few(Mm8Params p, const void *weights, const void *x, int width, cudaStream_t st) {
+    using L = Few<NT>;
+    const int row_tiles = (p.rows + ROWS - 1) / ROWS, token_tiles = (p.tokens + NT - 1) / NT;
+    // Split the width while the CTAs still fit the SMs at once and every CTA keeps four blocks or more.
+    const long long slots = 148LL * L::CTAS, tiles = (long long)row_tiles * token_tiles;
+    int splits = 1;
+    while (splits < 8 && tiles * splits * 2 <= slots && p.blocks >= 8 * splits) splits *= 2;
+    p.splits = splits;
+    const CUtensorMap mw = codes_map(weights, width, p.rows, ROWS), mx = codes_map(x, width, p.tokens, NT);
+    launch_cluster(few_kernel<NT>, dim3(splits, row_tiles, token_tiles), L::THREADS, L::SMEM, splits, st, mw, mx, p);
 }
 
 }  // namespace
@@ -520,16 +583,15 @@ void mm8(float *out, const void *weights, const float *weight_scales, const void
         reserve(many_kernel, Many::SMEM);
     });
     Mm8Params p{out, weight_scales, scales, tokens, rows, (width + KB - 1) / KB, 1, 0, 0};
-    const long long big = (long long)((tokens + Many::MT - 1) / Many::MT) * ((rows + Many::NT - 1) / Many::NT);
-    if (tokens > 128 && big >= 100) {
-        p.m_tiles = (tokens + Many::MT - 1) / Many::MT;
-        p.tiles = (int)big;
+    const int m_tiles = (tokens + Many::MT - 1) / Many::MT;
+    const long long tiles = (long long)m_tiles * ((rows + Many::NT - 1) / Many::NT);
+    if (tokens > 128 && tiles >= 60) {
+        p.m_tiles = m_tiles;
+        p.tiles = (int)tiles;
         int dev = 0, sms = 148;
         if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
         const CUtensorMap mw = codes_map(weights, width, rows, Many::NT), mx = codes_map(x, width, tokens, Many::MT);
-        const cudaError_t e = launch_chained(many_kernel, dim3((unsigned)std::min<long long>(big, sms)), dim3(320), Many::SMEM, st,
-                                             mw, mx, p);
-        if (e != cudaSuccess) throw std::runtime_error(std::string("e4m3 product: ") + cudaGetErrorString(e));
+        launch_cluster(many_kernel, dim3((unsigned)std::min<long long>(tiles, sms)), Many::THREADS, Many::SMEM, 1, st, mw, mx, p);
     } else if (tokens <= 16) {
         launch_few<16>(p, weights, x, width, st);
     } else if (tokens <= 32) {
