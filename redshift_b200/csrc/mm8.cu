@@ -15,8 +15,8 @@
 //    shared memory in a fixed order, so that also few rows fill the SMs and no
 //    workspace or atomics are needed.
 //  * many_kernel (128 tokens as the MMA's M, 256 weight rows as its N): persistent
-//    CTAs.  Bound by the tensor pipe; with tokens in the TMEM lanes the two scales
-//    of a thread's columns are one factor per block.
+//    CTAs.  With tokens in the TMEM lanes the two scales of a thread's columns are
+//    one factor per block.  Bound by the way of a block's sums out of TMEM, see there.
 #include "common.cuh"
 #include "hotpath.h"
 
@@ -302,21 +302,23 @@ few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUte
 }
 
 // ---------------------------------------------------------------- many tokens
-// TMEM holds two blocks' sums (2 x 256 columns), so a block takes half of its
-// way from the MMA through the scaling warps and back.  What shortens that way:
-// the weight rows' halves go it separately, sixteen warps empty a block (64 sums
-// a thread; four warps on each scheduler hide the loads' latency), the scales are
-// in registers before the sums are there, and nobody else does the issuing
-// warps' work (copies of scales have a warp of their own).
+// A block's MMAs take 513 cycles, scaling and adding its 128 x 256 sums 256 cycles of
+// every FMA lane, and TMEM holds the sums of two blocks.  A block takes about 900
+// cycles: its sums' way from the MMA through two barriers and back, halved, and the
+// output of a tile, which waits for the stores.  Measured and not faster (4,001 x 5,120
+// x 17,408, beside this form's 390 us): pairs of CTAs on 256 x 256 tiles (cta_group::2)
+// 410-460, sixteen summing warps 400, halves of the weight rows handed over separately
+// 410, registers moved to the summing warps for two chunks in flight 410-450, rows of
+// the output by bulk copies 457.  Without the sums the MMAs of this shape run at 590
+// cycles a block.
 struct Many {
     static constexpr int MT = 128, NT = 256;                 // tokens, weight rows of a tile
-    static constexpr int STAGES = 4, BUFS = 2, SLOTS = STAGES + BUFS;
-    static constexpr int SUM_WARPS = 16, COLS = NT * 4 / SUM_WARPS, THREADS = 32 * (3 + SUM_WARPS), SCALE_WARP = 2 + SUM_WARPS;
+    static constexpr int STAGES = 4, BUFS = 2, SLOTS = STAGES + BUFS, SCALE_WARP = 10, THREADS = 352;
     static constexpr int X_BYTES = MT * KB, W_BYTES = NT * KB, STAGE = X_BYTES + W_BYTES;
     static constexpr int SLOT_FLOATS = MT + 4;
-    static constexpr int OUT_ROW = 12;                       // floats of a staged row: 8 columns and a pad
-    static constexpr int SM_OUT = STAGES * STAGE;            // [SUM_WARPS][32 rows][OUT_ROW]
-    static constexpr int SM_SCALE = SM_OUT + SUM_WARPS * 32 * OUT_ROW * 4;
+    static constexpr int OUT_ROW = 20;                       // floats of a staged row: 16 columns and a pad
+    static constexpr int SM_OUT = STAGES * STAGE;            // [8 warps][32 rows][OUT_ROW]
+    static constexpr int SM_SCALE = SM_OUT + 8 * 32 * OUT_ROW * 4;
     static constexpr int SM_BAR = SM_SCALE + SLOTS * SLOT_FLOATS * 4;
     static constexpr int SMEM = SM_BAR + 256;
     static_assert(SMEM <= 227 * 1024, "shared memory of a CTA");
@@ -327,17 +329,17 @@ many_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUt
     using L = Many;
     extern __shared__ __align__(1024) uint8_t smem[];
     uint64_t *full = reinterpret_cast<uint64_t *>(smem + L::SM_BAR), *empty = full + L::STAGES;
-    uint64_t *d_full = empty + L::STAGES, *d_empty = d_full + 2 * L::BUFS, *s_full = d_empty + 2 * L::BUFS;   // d: [buffer][half]
+    uint64_t *d_full = empty + L::STAGES, *d_empty = d_full + L::BUFS, *s_full = d_empty + L::BUFS;
     uint64_t *mma_done = s_full + L::SLOTS;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(mma_done + 1);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
     float *slots = reinterpret_cast<float *>(smem + L::SM_SCALE);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const bool bad_base = (smem_addr(smem) & 1023) != 0;      // 128B-swizzle atoms need a 1024-byte aligned base
+    const bool bad_base = (smem_addr(smem) & 1023) != 0;
     if (threadIdx.x == 0) {
         for (int i = 0; i < L::STAGES; ++i) { mbar_init(full + i, 1); mbar_init(empty + i, 1); }
-        for (int i = 0; i < 2 * L::BUFS; ++i) { mbar_init(d_full + i, 1); mbar_init(d_empty + i, L::SUM_WARPS / 2); }
+        for (int i = 0; i < L::BUFS; ++i) { mbar_init(d_full + i, 1); mbar_init(d_empty + i, 8); }
         for (int i = 0; i < L::SLOTS; ++i) mbar_init(s_full + i, 32);
         mbar_init(mma_done, 1);
         *abort_flag = bad_base ? 1 : 0;
@@ -384,34 +386,6 @@ many_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUt
             for (int q = max(0, j - L::STAGES); q < j; ++q)
                 while (!mbar_try_wait(full + q % L::STAGES, (q / L::STAGES) & 1) && clock64() - start < WAIT_LIMIT_CYCLES) {}
         }
-    } else if (warp == 1) {
-        // ------------------------------------------------ MMA issuer
-        constexpr uint32_t idesc = idesc_e4m3(L::MT, L::NT / 2);
-        const uint32_t lead = elect_lane(), tm = __shfl_sync(0xffffffffu, tmem, 0);
-        const int n = mine * p.blocks;
-        for (int j = 0, s = 0, lap = 0; j < n; ++j) {
-            const int d = j & 1;
-            if (!warp_wait8(full + s, lap & 1, abort_flag)) break;
-            const uint64_t x = sw128_desc(smem_addr(smem + s * L::STAGE), 16, 1024);
-            const uint64_t w = sw128_desc(smem_addr(smem + s * L::STAGE + L::X_BYTES), 16, 1024);
-            bool ok = true;
-            for (int h = 0; h < 2; ++h) {
-                ok = j < 2 || warp_wait8(d_empty + 2 * d + h, ((j >> 1) - 1) & 1, abort_flag);
-                if (!ok) break;
-                tc_fence_after();
-#pragma unroll
-                for (int k = 0; k < KB / 32; ++k)
-                    mma_e4m3_ss_by(lead, tm + d * L::NT + h * (L::NT / 2), x + 2 * k, w + h * (L::W_BYTES / 32) + 2 * k, idesc,
-                                   k > 0 ? 1u : 0u);
-                mma_commit_by(lead, d_full + 2 * d + h);
-            }
-            if (!ok) break;
-            mma_commit_by(lead, empty + s);
-            if (++s == L::STAGES) { s = 0; ++lap; }
-        }
-        mma_commit_by(lead, mma_done);
-        const long long start = clock64();
-        while (!mbar_try_wait(mma_done, 0) && clock64() - start < WAIT_LIMIT_CYCLES) {}
     } else if (warp == L::SCALE_WARP) {
         // ------------------------------------------------ scales, by small copies
         int s = 0, lap = 0, slot = 0;
@@ -444,59 +418,80 @@ many_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUt
             }
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
+    } else if (warp == 1) {
+        constexpr uint32_t idesc = idesc_e4m3(L::MT, L::NT);
+        const uint32_t lead = elect_lane(), tm = __shfl_sync(0xffffffffu, tmem, 0);
+        const int n = mine * p.blocks;
+        for (int j = 0, s = 0, lap = 0; j < n; ++j) {
+            const int d = j & 1;
+            if (!warp_wait8(full + s, lap & 1, abort_flag)) break;
+            if (j >= 2 && !warp_wait8(d_empty + d, ((j >> 1) - 1) & 1, abort_flag)) break;
+            tc_fence_after();
+            const uint64_t x = sw128_desc(smem_addr(smem + s * L::STAGE), 16, 1024);
+            const uint64_t w = sw128_desc(smem_addr(smem + s * L::STAGE + L::X_BYTES), 16, 1024);
+#pragma unroll
+            for (int k = 0; k < KB / 32; ++k)
+                mma_e4m3_ss_by(lead, tm + d * L::NT, x + 2 * k, w + 2 * k, idesc, k > 0 ? 1u : 0u);
+            mma_commit_by(lead, empty + s);
+            mma_commit_by(lead, d_full + d);
+            if (++s == L::STAGES) { s = 0; ++lap; }
+        }
+        mma_commit_by(lead, mma_done);
+        const long long start = clock64();
+        while (!mbar_try_wait(mma_done, 0) && clock64() - start < WAIT_LIMIT_CYCLES) {}
     } else {
-        // ------------------------------------------------ sums
-        // Four warps a quarter of TMEM's lanes, 64 columns each; thread = lane = token.
-        const int group = (warp - 2) >> 2, half = group >> 1, lrow = (warp & 3) * 32;
-        const uint32_t t_col = tmem + ((uint32_t)lrow << 16) + group * L::COLS;
+        // Warps 2-5 take the tile's columns [0, 128), warps 6-9 [128, 256);
+        // thread = TMEM lane = token.
+        const int half = (warp - 2) >> 2, lrow = (warp & 3) * 32;
+        const uint32_t t_col = tmem + ((uint32_t)lrow << 16) + half * 128;
         float *stage = reinterpret_cast<float *>(smem + L::SM_OUT) + (warp - 2) * 32 * L::OUT_ROW;
-        const bool vec = p.rows % 4 == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15) == 0;
-        int j = 0, slot = 0, slap = 0;
+        int j = 0;
         bool ok = true;
         for (int i = 0; i < mine && ok; ++i) {
             const int tile = blockIdx.x + i * gridDim.x, m0 = tile % p.m_tiles * L::MT, n0 = tile / p.m_tiles * L::NT;
-            float2 acc[L::COLS / 2];
+            float2 acc[64];
 #pragma unroll
-            for (int c = 0; c < L::COLS / 2; ++c) acc[c] = make_float2(0.f, 0.f);
+            for (int c = 0; c < 64; ++c) acc[c] = make_float2(0.f, 0.f);
             for (int b = 0; b < p.blocks; ++b, ++j) {
-                const int d = j & 1;
-                if (!warp_wait8(s_full + slot, slap & 1, abort_flag)) { ok = false; break; }
+                const int d = j % L::BUFS, slot = j % L::SLOTS;
+                if (!warp_wait8(s_full + slot, (j / L::SLOTS) & 1, abort_flag) ||
+                    !warp_wait8(d_full + d, (j / L::BUFS) & 1, abort_flag)) { ok = false; break; }
+                tc_fence_after();
                 const float *sc = slots + slot * L::SLOT_FLOATS;
                 const float f = sc[lrow + lane] * sc[L::MT + half];
                 const float2 f2 = make_float2(f, f);
-                if (!warp_wait8(d_full + 2 * d + half, (j >> 1) & 1, abort_flag)) { ok = false; break; }
-                tc_fence_after();
+                float x[2][16];
 #pragma unroll
-                for (int c0 = 0; c0 < L::COLS; c0 += 16) {
-                    float x[16];
-                    tmem_ld16(t_col + d * L::NT + c0, x);
+                for (int c0 = 0; c0 < 128; c0 += 32) {
+                    tmem_ld16(t_col + d * L::NT + c0, x[0]);
+                    tmem_ld16(t_col + d * L::NT + c0 + 16, x[1]);
                     tmem_wait_ld();
-                    if (c0 + 16 == L::COLS) {
-                        tc_fence_before();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(d_empty + 2 * d + half);
-                    }
 #pragma unroll
-                    for (int c = 0; c < 8; ++c)
-                        acc[c0 / 2 + c] = ffma2(make_float2(x[2 * c], x[2 * c + 1]), f2, acc[c0 / 2 + c]);
+                    for (int q = 0; q < 2; ++q)
+#pragma unroll
+                        for (int c = 0; c < 8; ++c)
+                            acc[c0 / 2 + q * 8 + c] = ffma2(make_float2(x[q][2 * c], x[q][2 * c + 1]), f2, acc[c0 / 2 + q * 8 + c]);
                 }
-                if (++slot == L::SLOTS) { slot = 0; ++slap; }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(d_empty + d);
             }
             if (!ok) break;
-            // 8 columns at a time through shared memory: whole 32-byte sectors of sixteen rows per store.
+            // 16 columns at a time through shared memory: 64-byte pieces of eight rows per store.
+            const bool vec = p.rows % 4 == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15) == 0;
 #pragma unroll
-            for (int c0 = 0; c0 < L::COLS; c0 += 8) {
+            for (int c0 = 0; c0 < 128; c0 += 16) {
 #pragma unroll
-                for (int c = 0; c < 8; c += 4) {
+                for (int c = 0; c < 16; c += 4) {
                     const float2 a = acc[(c0 + c) / 2], e = acc[(c0 + c) / 2 + 1];
                     *reinterpret_cast<float4 *>(stage + lane * L::OUT_ROW + c) = make_float4(a.x, a.y, e.x, e.y);
                 }
                 __syncwarp();
-                const int col = n0 + group * L::COLS + c0 + (lane & 1) * 4;
+                const int col = n0 + half * 128 + c0 + (lane & 3) * 4;
 #pragma unroll
-                for (int r0 = 0; r0 < 32; r0 += 16) {
-                    const int r = r0 + (lane >> 1), token = m0 + lrow + r;
-                    const float4 v = *reinterpret_cast<const float4 *>(stage + r * L::OUT_ROW + (lane & 1) * 4);
+                for (int r0 = 0; r0 < 32; r0 += 8) {
+                    const int r = r0 + (lane >> 2), token = m0 + lrow + r;
+                    const float4 v = *reinterpret_cast<const float4 *>(stage + r * L::OUT_ROW + (lane & 3) * 4);
                     if (token >= p.tokens) continue;
                     float *dst = p.out + (size_t)token * p.rows + col;
                     if (vec) {
@@ -564,10 +559,12 @@ void launch_cluster(K *kernel, dim3 grid, int threads, int smem, int cluster, cu
 template <int NT> void launch_few(Mm8Params p, const void *weights, const void *x, int width, cudaStream_t st) {
     using L = Few<NT>;
     const int row_tiles = (p.rows + ROWS - 1) / ROWS, token_tiles = (p.tokens + NT - 1) / NT;
-    // Split the width while the CTAs still fit the SMs at once and every CTA keeps four blocks or more.
+    // Split the width as far as the CTAs fit the SMs at once and every CTA keeps four
+    // blocks, but not over clusters of more than six: seven and eight pack badly (1 x
+    // 6,144 x 5,120: four 9.6, six 10.0, seven 16.3, eight 15.6 us; 64 x 5,120 x
+    // 10,240: two 17.6, three 15.6; 100 x 5,120 x 5,120: two 16.0, three 13.7).
     const long long slots = 148LL * L::CTAS, tiles = (long long)row_tiles * token_tiles;
-    int splits = 1;
-    while (splits < 8 && tiles * splits * 2 <= slots && p.blocks >= 8 * splits) splits *= 2;
+    const int splits = (int)std::max(1LL, std::min<long long>({6, slots / tiles, p.blocks / 4}));
     p.splits = splits;
     const CUtensorMap mw = codes_map(weights, width, p.rows, ROWS), mx = codes_map(x, width, p.tokens, NT);
     launch_cluster(few_kernel<NT>, dim3(splits, row_tiles, token_tiles), L::THREADS, L::SMEM, splits, st, mw, mx, p);
@@ -585,7 +582,11 @@ void mm8(float *out, const void *weights, const float *weight_scales, const void
     Mm8Params p{out, weight_scales, scales, tokens, rows, (width + KB - 1) / KB, 1, 0, 0};
     const int m_tiles = (tokens + Many::MT - 1) / Many::MT;
     const long long tiles = (long long)m_tiles * ((rows + Many::NT - 1) / Many::NT);
-    if (tokens > 128 && tiles >= 60) {
+    // Beyond 128 tokens few_kernel<128> is still the faster one while all its tiles
+    // run at once (384 x 5,120 x 5,120: 24.1 against 27.1 us, 256 x 17,408 x 5,120: 65
+    // against 72; two waves of it, 256 x 5,120 x 10,240: 42 against 28).
+    const long long few_tiles = (long long)((tokens + 127) / 128) * ((rows + ROWS - 1) / ROWS);
+    if (tokens > 128 && few_tiles > 148) {
         p.m_tiles = m_tiles;
         p.tiles = (int)tiles;
         int dev = 0, sms = 148;
