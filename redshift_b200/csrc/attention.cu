@@ -143,7 +143,7 @@ fa_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
     prepare_queries<false>(p, kv_head, rope, smem + L::SM_P, tmem, q_ready, [&] { issue_early(0, early); }, unused);
     if ((warp == 2 || warp == 3) && appends) {
         // The new rows become visible to the TMA loads of this CTA.
-        append_rows<false>(p, kv_head, warp - 2, app_lo, app_hi, rope, [](int row) { return row; });
+        append_rows(p, kv_head, warp - 2, app_lo, app_hi, rope);
         fence_async_global();
         mbar_arrive(app_done);
     }

@@ -94,6 +94,60 @@ template <bool VALUES> __device__ __forceinline__ uint4 fp16_codes(uint32_t a, u
                       fp16_pair<VALUES>(b, 0x4342));
 }
 
+// Append (converter warps, positions pos, pos + 8, ... below `end`): RMSNorm +
+// rotary of the new keys, fp16 keys and values into the ring.  What lands in the
+// cache is read by every later token, so the keys are formed in 64 bits and
+// rounded once (in 32 bits a value near a border of two fp16 numbers now and then
+// went to the further one); the warps are idle meanwhile.  Returns the tokens, as
+// bits, whose fp16 values are not all finite.
+__device__ __forceinline__ uint32_t append_row8(const FaParams &p, int ring, int kv_head, int pos, int end) {
+    const int lane = threadIdx.x & 31;
+    uint32_t bad = 0;
+#pragma unroll 1
+    for (; pos < end; pos += 2 * CONV_WARPS) {
+        const int t = pos - p.position;
+        const size_t src = ((size_t)t * NKV + kv_head) * HD + 4 * lane, dst = ((size_t)(pos % ring) * NKV + kv_head) * HD + 4 * lane;
+        float k[8], w[8], v[8];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            *reinterpret_cast<float4 *>(k + 4 * h) = *reinterpret_cast<const float4 *>(p.key + src + 128 * h);
+            *reinterpret_cast<float4 *>(w + 4 * h) = *reinterpret_cast<const float4 *>(p.kn + 4 * lane + 128 * h);
+            *reinterpret_cast<float4 *>(v + 4 * h) = *reinterpret_cast<const float4 *>(p.value + src + 128 * h);
+        }
+        double ss = 0., x[8], cosine, sine;
+        sincospi((double)pos * kRopeInvFreq[lane] * 0.3183098861837907, &sine, &cosine);      // angle of dims lane, lane + 32
+#pragma unroll
+        for (int e = 0; e < 8; ++e) ss = fma((double)k[e], (double)k[e], ss);
+#pragma unroll
+        for (int o = 16; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        const double inv = rsqrt(ss / HD + (double)p.eps);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = (double)k[e] * inv * (double)w[e];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {                          // dims 4 lane + e: lanes 0..7 pair with 8..15
+            const double partner = __shfl_xor_sync(0xffffffffu, x[e], 8);
+            const double c = __shfl_sync(0xffffffffu, cosine, 4 * (lane & 7) + e), s = __shfl_sync(0xffffffffu, sine, 4 * (lane & 7) + e);
+            if (lane < 16) x[e] = fma(partner, lane < 8 ? -s : s, x[e] * c);
+        }
+        bool finite = true;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            __half2 kh[2], vh[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                kh[e] = __halves2half2(__double2half(x[4 * h + 2 * e]), __double2half(x[4 * h + 2 * e + 1]));
+                vh[e] = __floats2half2_rn(v[4 * h + 2 * e], v[4 * h + 2 * e + 1]);
+                const float2 f = __half22float2(__habs2(vh[e]));
+                finite = finite && f.x <= 65504.f && f.y <= 65504.f;
+            }
+            *reinterpret_cast<uint2 *>(p.kc + dst + 128 * h) = make_uint2(half2_bits(kh[0]), half2_bits(kh[1]));
+            *reinterpret_cast<uint2 *>(p.vc + dst + 128 * h) = make_uint2(half2_bits(vh[0]), half2_bits(vh[1]));
+        }
+        if (!__all_sync(0xffffffffu, finite)) bad |= 1u << t;
+    }
+    return bad;
+}
+
 __global__ void __launch_bounds__(THREADS8, 1) attention8_kernel(const FaParams p, const Cache8View c) {
     using L = A8Layout;
     extern __shared__ __align__(1024) uint8_t smem[];
@@ -133,7 +187,7 @@ __global__ void __launch_bounds__(THREADS8, 1) attention8_kernel(const FaParams 
         mbar_init(mma_done, 1);
         mbar_init(q_ready, 8);
         mbar_init(cbar, 1);
-        mbar_init(app_done, 64);
+        mbar_init(app_done, 2 * CONV_WARPS * 32);
         mbar_init(q_loaded, 1);
         for (int i = 0; i < 8; ++i) mbar_init(maximum_of + i, 1);
         *abort_flag = 0;
@@ -201,6 +255,12 @@ __global__ void __launch_bounds__(THREADS8, 1) attention8_kernel(const FaParams 
             __syncwarp();
             if (lane == 0) mbar_arrive(bar);
         };
+        if (appends) {                                        // while the first tiles are on their way
+            const uint32_t bad = append_row8(p, c.ring, kv_head, app_lo + (warp - SOFT_WARPS), app_hi);
+            if (lane == 0 && bad) atomicOr(bad_values, bad);
+            __threadfence_block();
+            mbar_arrive(app_done);
+        }
         uint64_t *full = part ? v_full : k_full, *empty = part ? v_empty : k_empty;
         const __half *rows = part ? p.vc : p.kc;
         for (int j = 0, slot = 0, lap = 0; j < ntiles; ++j) {
@@ -308,13 +368,6 @@ __global__ void __launch_bounds__(THREADS8, 1) attention8_kernel(const FaParams 
     }
     float row_sums[QR];
     prepare_queries<true>(p, kv_head, rope, smem + L::SM_QSTAGE, tmem, q_ready, [&] { mbar_arrive(q_loaded); }, row_sums);
-    if ((warp == 2 || warp == 3) && appends) {
-        const int ring = c.ring;
-        const uint32_t bad = append_rows<true>(p, kv_head, warp - 2, app_lo, app_hi, rope, [ring](int pos) { return pos % ring; });
-        if (lane == 0 && bad) atomicOr(bad_values, bad);
-        __threadfence_block();
-        mbar_arrive(app_done);
-    }
     {
         // ------------------------------------------------ softmax
         // Lanes 32g + i and 32g + 16 + i of TMEM hold the hi and lo halves of query
@@ -328,7 +381,7 @@ __global__ void __launch_bounds__(THREADS8, 1) attention8_kernel(const FaParams 
         float m_use[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 #pragma unroll
         for (int u = 0; u < 2; ++u) last[u] = r0 + 8 * u < rows ? p.position + (r0 + 8 * u) / GROUP : -1;
-        // Once the append has used the rotary table, its place takes the queries'
+        // Once the queries are rotated, the rotary table's place takes the queries'
         // sums (row warp + 8 j), the scales and the running maxima.
         float *maxima = reinterpret_cast<float *>(rope);           // [tile parity][64 rows]
         float *sums = maxima + 2 * DECODE_ROWS, *scales = sums + DECODE_ROWS, bias[2];

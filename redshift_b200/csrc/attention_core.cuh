@@ -528,19 +528,14 @@ __device__ __forceinline__ void prepare_queries(const FaParams &p, int kv_head, 
     }
 }
 
-// Append (one of two warps, k = 0 or 1): RMSNorm + rotary of the new keys, fp16
-// keys / values of the cache rows [lo, hi) of this CTA's tiles, row r at row
-// dst_row(r) of the caches.  CHECK: returns the tokens, as bits, whose fp16
-// values are not all finite.
-template <bool CHECK, class Row>
-__device__ __forceinline__ uint32_t append_rows(const FaParams &p, int kv_head, int k, int lo, int hi, const float2 *rope,
-                                                Row &&dst_row) {
+// The rows a decode launch appends: RMSNorm + rotary of the new keys, fp16 keys /
+// values of the cache rows [lo, hi) of this CTA's tiles, one of two warps (k = 0 or 1).
+__device__ __forceinline__ void append_rows(const FaParams &p, int kv_head, int k, int lo, int hi, const float2 *rope) {
     const int lane = threadIdx.x & 31;
-    uint32_t bad = 0;
     const float4 k0 = *reinterpret_cast<const float4 *>(p.kn + 4 * lane);
     const float4 k1 = *reinterpret_cast<const float4 *>(p.kn + 128 + 4 * lane);
     for (int row = lo + k; row < hi; row += 2) {
-        const int tt = row - p.append_row0, dst = dst_row(row);
+        const int tt = row - p.append_row0;
         const float *ks = p.key + ((size_t)tt * NKV + kv_head) * HD;
         const float *vs = p.value + ((size_t)tt * NKV + kv_head) * HD;
         const float4 a = *reinterpret_cast<const float4 *>(ks + 4 * lane);
@@ -553,24 +548,18 @@ __device__ __forceinline__ uint32_t append_rows(const FaParams &p, int kv_head, 
         const float inv = rsqrtf(sk / HD + p.eps);
         float x0[4] = {a.x * inv * k0.x, a.y * inv * k0.y, a.z * inv * k0.z, a.w * inv * k0.w};
         rope_row(x0, rope + tt * 32, lane, true);
-        __half *kd = p.kc + ((size_t)dst * NKV + kv_head) * HD;
-        __half *vd = p.vc + ((size_t)dst * NKV + kv_head) * HD;
+        __half *kd = p.kc + ((size_t)row * NKV + kv_head) * HD;
+        __half *vd = p.vc + ((size_t)row * NKV + kv_head) * HD;
         *reinterpret_cast<uint2 *>(kd + 4 * lane) =
             make_uint2(half2_bits(__floats2half2_rn(x0[0], x0[1])), half2_bits(__floats2half2_rn(x0[2], x0[3])));
         *reinterpret_cast<uint2 *>(kd + 128 + 4 * lane) =
             make_uint2(half2_bits(__floats2half2_rn(b.x * inv * k1.x, b.y * inv * k1.y)),
                        half2_bits(__floats2half2_rn(b.z * inv * k1.z, b.w * inv * k1.w)));
-        const __half2 v0 = __floats2half2_rn(va.x, va.y), v1 = __floats2half2_rn(va.z, va.w);
-        const __half2 v2 = __floats2half2_rn(vb.x, vb.y), v3 = __floats2half2_rn(vb.z, vb.w);
-        *reinterpret_cast<uint2 *>(vd + 4 * lane) = make_uint2(half2_bits(v0), half2_bits(v1));
-        *reinterpret_cast<uint2 *>(vd + 128 + 4 * lane) = make_uint2(half2_bits(v2), half2_bits(v3));
-        if (CHECK) {
-            const __half2 top = __hmax2_nan(__hmax2_nan(__habs2(v0), __habs2(v1)), __hmax2_nan(__habs2(v2), __habs2(v3)));
-            const float2 f = __half22float2(top);
-            if (__any_sync(0xffffffffu, !(f.x <= 65504.f) || !(f.y <= 65504.f))) bad |= 1u << tt;
-        }
+        *reinterpret_cast<uint2 *>(vd + 4 * lane) =
+            make_uint2(half2_bits(__floats2half2_rn(va.x, va.y)), half2_bits(__floats2half2_rn(va.z, va.w)));
+        *reinterpret_cast<uint2 *>(vd + 128 + 4 * lane) =
+            make_uint2(half2_bits(__floats2half2_rn(vb.x, vb.y)), half2_bits(__floats2half2_rn(vb.z, vb.w)));
     }
-    return bad;
 }
 
 // Epilogue of a decode CTA (its first 8 warps), once O is complete and the K/V

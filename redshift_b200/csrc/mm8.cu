@@ -11,7 +11,7 @@
 // Two kernels:
 //  * few_kernel<NT> (tokens as the MMA's N, 16..128 of them): 128 weight rows
 //    per CTA.  Bound by reading the weights once from HBM; the width is split
-//    over a cluster of up to 8 CTAs whose partial sums meet in distributed
+//    over a cluster of up to six CTAs whose partial sums meet in distributed
 //    shared memory in a fixed order, so that also few rows fill the SMs and no
 //    workspace or atomics are needed.
 //  * many_kernel (128 tokens as the MMA's M, 256 weight rows as its N): persistent
@@ -31,7 +31,7 @@ constexpr int KB = 128;                        // columns of a block = one 128-b
 constexpr int ROWS = 128;                      // weight rows that share a scale
 
 // D[tmem] (+)= A[smem] * B[smem]^T for e4m3 codes, fp32 accumulate, K = 32;
-// issued by a whole warp, one elected lane (see mma_f16_ss_by).
+// issued by a whole warp, one elected lane (see mma_f16_ts_by).
 __device__ __forceinline__ void mma_e4m3_ss_by(uint32_t elected, uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
                                                uint32_t idesc, uint32_t accumulate) {
     asm volatile("{\n\t.reg .pred p, q;\n\t"
