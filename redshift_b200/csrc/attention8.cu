@@ -10,12 +10,19 @@
 // tile of 64 positions is one block, so its two scales are one factor of its
 // scores and one of its probabilities.
 //
-// Bound by the cache's bytes, 2 KB a position.  What keeps the tensor cores fed
-// at twice the fp16 cache's tile rate:
+// The floor is the cache's bytes, 2 KB a position: 8 tokens at 139,256 take 71 us
+// (4.0 TB/s, 390 TFLOP/s of products, 44 us at the copy rate), 5 at 32,767 28 us, 1
+// at 777 12 us; the fp16 cache's kernel takes 101 us for the longest.  What bounds
+// it is what a tile moves through shared memory (fp16 images written 64 KB and
+// read 64 KB by the MMAs, codes 32 KB: half as much again when the codes were
+// staged there too, 73 us) and, in calls without a pause, the power limit: 990 W
+// and 1.5 GHz, 86 us.  About 12 us of a call are its two ends: 4 us to the first
+// tile, 8 us from the last one through the splits' combination.
+// What keeps the tensor cores fed at twice the fp16 cache's tile rate:
 //  * eight converter warps (four for K, four for V) write the codes as exact fp16
-//    numbers into the MMA's swizzled operand images.  A producer warp keeps three
-//    tiles of K and of V on their way in shared memory (96 KB per SM; a block of
-//    one head is 16 KB in a row, one bulk copy);
+//    numbers into the MMA's swizzled operand images.  They ask for the next tile's
+//    codes, straight into registers, as soon as this tile's are written; bulk
+//    prefetches into L2 run AHEAD tiles before that;
 //  * the eight warps that prepared the queries are the softmax, two for each
 //    quarter of TMEM's lanes, which take the tiles in turn: a tile's latency from
 //    its scores to its probabilities is longer than its share of the time, and
@@ -47,27 +54,37 @@ namespace qv {
 namespace {
 
 constexpr int IMAGES = 2;        // fp16 tile images (K and V each)
-constexpr int RAW_SLOTS = 3;     // code tiles in flight (K and V each)
+constexpr int AHEAD = 4;         // code tiles on their way into L2 (K and V each)
 constexpr int WARP_ROWS = 16;    // a converter warp's rows of a tile
-constexpr int SOFT_WARPS = 8, CONV_WARPS = 4, MMA_WARP = SOFT_WARPS + 2 * CONV_WARPS, PRODUCER_WARP = MMA_WARP + 1;
-constexpr int THREADS8 = 32 * (PRODUCER_WARP + 1);
+constexpr int SOFT_WARPS = 8, CONV_WARPS = 4, MMA_WARP = SOFT_WARPS + 2 * CONV_WARPS;
+constexpr int THREADS8 = 32 * (MMA_WARP + 1);
 constexpr int CODES_TILE = BN * HD;                               // codes of one (block, head)
 constexpr int MAX_TILES8 = 160;  // tiles of a CTA (59 at the longest context on 148 SMs)
 constexpr float P_BIAS = 6.f;    // log2 units above the running maximum
 struct A8Layout {
     static constexpr int SM_KV = 0;                               // images: (K, V) of two tiles
     static constexpr int SM_KV_STAGE = 2 * TILE_BYTES;
-    static constexpr int SM_RAW = SM_KV + IMAGES * SM_KV_STAGE;   // code tiles [slot][K, V]
-    static constexpr int SM_QSTAGE = SM_RAW + 4 * CODES_TILE;     // slot 2 until the queries are in TMEM
-    static constexpr int SM_BAR = SM_RAW + RAW_SLOTS * 2 * CODES_TILE;
+    static constexpr int SM_QSTAGE = EPILOGUE_BYTES;              // the queries on their way to TMEM, then the tail's scratch
+    static constexpr int SM_BAR = SM_QSTAGE + 2 * DECODE_ROWS * 256;
     static constexpr int SM_ROPE = SM_BAR + 384;                  // (cos, sin) [T][32]; then maxima, sums and scales
     static constexpr int SMEM_BYTES = SM_ROPE + MAX_DECODE_T * 32 * 8;
     static_assert((3 * DECODE_ROWS + 2 * MAX_TILES8) * 4 <= MAX_DECODE_T * 32 * 8);
 };
 static_assert(A8Layout::SMEM_BYTES <= 227 * 1024, "attention kernel exceeds the shared memory of a CTA");
-static_assert(EPILOGUE_BYTES <= A8Layout::SM_BAR, "O staging exceeds the images and the ring");
+static_assert(IMAGES * A8Layout::SM_KV_STAGE <= A8Layout::SM_QSTAGE, "the images overlap the staged queries");
 static_assert(BN == CACHE8_BLOCK, "a tile is a block of the cache");
 
+// A tile's codes are read once by this SM: not kept in L1.
+__device__ __forceinline__ uint4 ld_once(const uint4 *a) {
+    uint4 v;
+    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(a) : "memory");
+    return v;
+}
+// `bytes` (a multiple of 16) on their way into L2.
+__device__ __forceinline__ void prefetch_l2_bulk(const void *a, uint32_t bytes) {
+    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" :: "l"(a), "r"(bytes) : "memory");
+}
 struct Cache8View {
     const int8_t *kc, *vc;       // codes [block][4][64][256]
     const float *ks, *vs;        // scales [block][4]
@@ -155,10 +172,9 @@ __global__ void __launch_bounds__(THREADS8, 1) attention8_kernel(const FaParams 
         if (threadIdx.x == 0) raise_status(STATUS_BAD_ARGUMENT);
         return;
     }
-    uint64_t *raw_full = reinterpret_cast<uint64_t *>(smem + L::SM_BAR), *raw_empty = raw_full + 2 * RAW_SLOTS;   // [K, V][slot]
-    uint64_t *k_full = raw_empty + 2 * RAW_SLOTS, *v_full = k_full + 2, *k_empty = k_full + 4, *v_empty = k_full + 6,
-             *s_full = k_full + 8, *p_full = k_full + 10, *p_free = k_full + 12, *mma_done = k_full + 14,
-             *q_ready = k_full + 15, *app_done = k_full + 16, *cbar = k_full + 17, *q_loaded = k_full + 18, *maximum_of = k_full + 19;  // 39 in all
+    uint64_t *k_full = reinterpret_cast<uint64_t *>(smem + L::SM_BAR), *v_full = k_full + 2, *k_empty = k_full + 4,
+             *v_empty = k_full + 6, *s_full = k_full + 8, *p_full = k_full + 10, *p_free = k_full + 12, *mma_done = k_full + 14,
+             *q_ready = k_full + 15, *app_done = k_full + 16, *cbar = k_full + 17, *q_loaded = k_full + 18, *maximum_of = k_full + 19;  // 27 in all
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + L::SM_BAR + 320);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(smem + L::SM_BAR + 324);
     uint32_t *bad_values = reinterpret_cast<uint32_t *>(smem + L::SM_BAR + 328);
@@ -178,17 +194,16 @@ __global__ void __launch_bounds__(THREADS8, 1) attention8_kernel(const FaParams 
         prefetch_l2(p.q_gate + ((size_t)(rr / GROUP) * NQ + kv_head * GROUP + rr % GROUP) * 2 * HD + (i & 7) * 32);
     }
     if (threadIdx.x == 0) {
-        for (int i = 0; i < 2 * RAW_SLOTS; ++i) { mbar_init(raw_full + i, 1); mbar_init(raw_empty + i, CONV_WARPS); }
         for (int i = 0; i < 2; ++i) {
             mbar_init(k_full + i, CONV_WARPS); mbar_init(v_full + i, CONV_WARPS);
             mbar_init(k_empty + i, 1); mbar_init(v_empty + i, 1);
             mbar_init(s_full + i, 1); mbar_init(p_full + i, SOFT_WARPS / 2); mbar_init(p_free + i, 1);
         }
         mbar_init(mma_done, 1);
+        mbar_init(q_loaded, 1);
         mbar_init(q_ready, 8);
         mbar_init(cbar, 1);
         mbar_init(app_done, 2 * CONV_WARPS * 32);
-        mbar_init(q_loaded, 1);
         for (int i = 0; i < 8; ++i) mbar_init(maximum_of + i, 1);
         *abort_flag = 0;
         *bad_values = 0;
@@ -207,7 +222,7 @@ __global__ void __launch_bounds__(THREADS8, 1) attention8_kernel(const FaParams 
     if (warp >= SOFT_WARPS && warp < MMA_WARP) {
         // ------------------------------------------------ converters (warps 8-11: K, 12-15: V)
         // A lane takes 16 codes (16 dims of a row) at a time: 16 bytes of the
-        // code tile, two 16-byte chunks of a 64-dim box of the image.  Eight
+        // block, two 16-byte chunks of a 64-dim box of the image.  Eight
         // lanes are four neighbouring pieces of an even row and four, in the
         // box's neighbour, of the odd row after it: their loads cover the two
         // halves of 128 bytes and their stores, swizzled by the row, even and
@@ -215,14 +230,19 @@ __global__ void __launch_bounds__(THREADS8, 1) attention8_kernel(const FaParams 
         const int part = (warp - SOFT_WARPS) >> 2, w = warp & 3, q = lane & 3, odd = lane >> 2 & 1;
         const int box = (lane >> 3) ^ odd, piece = 4 * box + q, row0 = WARP_ROWS * w + odd;
         const uint32_t image = box * (BN * 128) + row0 * 128;
-        const uint8_t *ring = smem + L::SM_RAW + part * CODES_TILE + row0 * HD + piece * 16;
-        uint64_t *landed = raw_full + part * RAW_SLOTS, *taken = raw_empty + part * RAW_SLOTS;
-        auto convert = [&](auto values, uint8_t *dst, int slot) {
-            constexpr bool V = decltype(values)::value;
-            uint4 x[8];
-            const uint8_t *src = ring + slot * 2 * CODES_TILE;
+        const int8_t *codes = (part ? c.vc : c.kc) + ((size_t)tile0 * NKV + kv_head) * CODES_TILE + WARP_ROWS * w * HD;
+        const size_t step = (size_t)NKV * CODES_TILE;
+        auto prefetch = [&](int j) {
+            if (lane == 0 && j < code_tiles) prefetch_l2_bulk(codes + j * step, WARP_ROWS * HD);
+        };
+        uint4 x[8];
+        auto load = [&](int j) {
+            const int8_t *src = codes + j * step + odd * HD + piece * 16;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = *reinterpret_cast<const uint4 *>(src + i * 2 * HD);
+            for (int i = 0; i < 8; ++i) x[i] = ld_once(reinterpret_cast<const uint4 *>(src + i * 2 * HD));
+        };
+        auto convert = [&](auto values, uint8_t *dst) {
+            constexpr bool V = decltype(values)::value;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 uint8_t *d = dst + image + i * 256;
@@ -263,61 +283,27 @@ __global__ void __launch_bounds__(THREADS8, 1) attention8_kernel(const FaParams 
         }
         uint64_t *full = part ? v_full : k_full, *empty = part ? v_empty : k_empty;
         const __half *rows = part ? p.vc : p.kc;
-        for (int j = 0, slot = 0, lap = 0; j < ntiles; ++j) {
+        // The first tiles are asked for once the query rows have arrived, which would
+        // wait behind them.
+        if (!warp_wait(q_loaded, 0, abort_flag)) return;
+        for (int i = 1; i < AHEAD; ++i) prefetch(i);
+        if (code_tiles > 0) load(0);
+        for (int j = 0; j < ntiles; ++j) {
             const int s = j & 1;
             uint8_t *dst = smem + L::SM_KV + s * L::SM_KV_STAGE + part * TILE_BYTES;
             const bool fresh = appends && (tile0 + j + 1) * BN > p.position;      // the tile holds new rows
-            if (j < code_tiles) {
-                if (!warp_wait(landed + slot, lap & 1, abort_flag)) break;
-            } else if (fresh && !warp_wait(app_done, 0, abort_flag)) {
-                break;
-            }
+            prefetch(j + AHEAD);
+            if (fresh && !warp_wait(app_done, 0, abort_flag)) break;
             if (j >= 2 && !warp_wait(empty + s, (uint32_t)((j >> 1) - 1) & 1, abort_flag)) break;
             if (j >= code_tiles) copy_rows(dst, rows, j, part && fresh ? *reinterpret_cast<volatile uint32_t *>(bad_values) : 0u);
-            else if (part) convert(std::true_type{}, dst, slot);
-            else convert(std::false_type{}, dst, slot);
+            else if (part) convert(std::true_type{}, dst);
+            else convert(std::false_type{}, dst);
+            if (j + 1 < code_tiles) load(j + 1);
             publish(full + s);
-            if (j < code_tiles && lane == 0) mbar_arrive(taken + slot);
-            if (++slot == RAW_SLOTS) { slot = 0; ++lap; }
         }
         return;                          // the later barriers count the first eight warps
     }
 
-    if (warp == PRODUCER_WARP) {
-        // ------------------------------------------------ producer
-        if (lane == 0 && code_tiles > 0) {
-            const size_t first = ((size_t)tile0 * NKV + kv_head) * CODES_TILE, step = (size_t)NKV * CODES_TILE;
-            const int8_t *src[2] = {c.kc + first, c.vc + first};
-            int issued = 0;                                   // halves: tile j's K is 2 j, its V 2 j + 1
-            // The first two tiles are asked for once the query rows have arrived
-            // (issued before them they would queue in front), the last slot once
-            // it stages no queries.
-            bool ok = mbar_wait(q_loaded, 0, abort_flag);
-            for (int j = 0, slot = 0, lap = 0; j < code_tiles && ok; ++j) {
-                if (j == RAW_SLOTS - 1) {
-                    ok = mbar_wait(q_ready, 0, abort_flag);
-                    fence_async_shared();                     // the staged queries were written and read by plain accesses
-                }
-#pragma unroll
-                for (int part = 0; part < 2; ++part) {
-                    uint64_t *bar = raw_full + part * RAW_SLOTS + slot;
-                    if (j >= RAW_SLOTS) ok = ok && mbar_wait(raw_empty + part * RAW_SLOTS + slot, (lap - 1) & 1, abort_flag);
-                    if (!ok) break;
-                    mbar_expect_tx(bar, CODES_TILE);
-                    bulk_load(smem + L::SM_RAW + (slot * 2 + part) * CODES_TILE, src[part], CODES_TILE, bar);
-                    src[part] += step;
-                    ++issued;
-                }
-                if (++slot == RAW_SLOTS) { slot = 0; ++lap; }
-            }
-            // Every issued copy must land before the CTA may exit.
-            const long long t0 = clock64();
-            for (int h = max(0, issued - 2 * RAW_SLOTS); h < issued; ++h)
-                while (!mbar_try_wait(raw_full + (h & 1) * RAW_SLOTS + (h >> 1) % RAW_SLOTS, (uint32_t)((h >> 1) / RAW_SLOTS) & 1) &&
-                       clock64() - t0 < WAIT_LIMIT_CYCLES) {}
-        }
-        return;
-    }
     if (warp == MMA_WARP) {
         // ------------------------------------------------ MMA issuer (the whole warp, one elected lane)
         const uint32_t lead = elect_lane(), tm = __shfl_sync(0xffffffffu, tmem, 0);
@@ -402,6 +388,14 @@ __global__ void __launch_bounds__(THREADS8, 1) attention8_kernel(const FaParams 
             // a scale of (almost) zero: its codes count nothing, its keys still do; NaN stays
             const float vs = scale.y < 0x1p-100f ? 0x1p-100f : scale.y;
             const float v_log2 = log2_approx(vs), v_inv = rcp_approx(vs);
+            // The running maximum of the tile before, from this row's other warp; its
+            // tile is half a round ahead, so that this costs nothing before the scores.
+            float before[2] = {-INFINITY, -INFINITY};
+            if (j > 0) {
+                if (!warp_wait(maximum_of + 2 * wq + (b ^ 1), ((j - 1) >> 1) & 1, abort_flag)) break;
+#pragma unroll
+                for (int u = 0; u < 2; ++u) before[u] = maxima[(b ^ 1) * DECODE_ROWS + r0 + 8 * u];
+            }
             if (!warp_wait(s_full + b, (j >> 1) & 1, abort_flag)) break;
             tc_fence_after();
             float2 x[16];
@@ -436,8 +430,11 @@ __global__ void __launch_bounds__(THREADS8, 1) attention8_kernel(const FaParams 
                     x[q].y = masked(x[q].y, key0 + 8 * (q >> 1) + 1, q & 1);
                 }
             }
-            // The row's maximum: this thread's columns and the row's other three threads.
-            float m[2], before[2] = {-INFINITY, -INFINITY}, unbias[2];
+            // The largest of this thread's columns, in log2 units.  The running maximum
+            // moves only when a tile's is far above it, so that most tiles need no
+            // more than this and a vote.
+            float m[2], unbias[2];
+            bool above = false;
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
                 float m0 = fmaxf(x[u].x, x[u].y), m1 = fmaxf(x[2 + u].x, x[2 + u].y);
@@ -446,27 +443,23 @@ __global__ void __launch_bounds__(THREADS8, 1) attention8_kernel(const FaParams 
                     m0 = fmaxf(m0, fmaxf(x[2 * n + u].x, x[2 * n + u].y));
                     m1 = fmaxf(m1, fmaxf(x[2 * n + 2 + u].x, x[2 * n + 2 + u].y));
                 }
-                m[u] = fmaxf(m0, m1);
-                m[u] = fmaxf(m[u], __shfl_xor_sync(0xffffffffu, m[u], 1));
-                m[u] = fmaxf(m[u], __shfl_xor_sync(0xffffffffu, m[u], 2));
                 unbias[u] = codes ? -bias[u] * score_log2 : 0.f;
-                m[u] = fmaf(m[u], to_log2, unbias[u] + v_log2);    // log2 units (-inf stays -inf)
+                m[u] = fmaf(fmaxf(m0, m1), to_log2, unbias[u] + v_log2);       // -inf stays -inf
+                above = above || m[u] > before[u] + RESCALE_THRESHOLD;
             }
-            // The running maximum of the tile before, from this row's other warp; it
-            // moves only when the tile's is far above it.
-            if (j > 0) {
-                if (!warp_wait(maximum_of + 2 * wq + (b ^ 1), ((j - 1) >> 1) & 1, abort_flag)) break;
+            const bool need = __any_sync(0xffffffffu, above);
+            if (need) {                                            // the rows' maxima: their other three threads
 #pragma unroll
-                for (int u = 0; u < 2; ++u) before[u] = maxima[(b ^ 1) * DECODE_ROWS + r0 + 8 * u];
-            }
-            bool need = false;
+                for (int u = 0; u < 2; ++u) {
+                    m[u] = fmaxf(m[u], __shfl_xor_sync(0xffffffffu, m[u], 1));
+                    m[u] = fmaxf(m[u], __shfl_xor_sync(0xffffffffu, m[u], 2));
+                    m[u] = m[u] > before[u] + RESCALE_THRESHOLD ? m[u] : before[u];
+                }
+            } else {
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const bool raise = m[u] > before[u] + RESCALE_THRESHOLD;
-                need = need || raise;
-                m[u] = raise ? m[u] : before[u];
+                for (int u = 0; u < 2; ++u) m[u] = before[u];
             }
-            if (j > 0 && __any_sync(0xffffffffu, need)) {
+            if (j > 0 && need) {
                 // O holds the tiles before j: wait for PV(j-1), then rescale its rows.
                 if (!warp_wait(p_free + (b ^ 1), ((j - 1) >> 1) & 1, abort_flag)) break;
                 tc_fence_after();
