@@ -9,7 +9,8 @@
 
 ``position`` is the caller's count of kept tokens: after a verify of 8 tokens of which 3 were kept
 the next call simply passes a position that is 3 higher.  Rows from ``position`` on are never
-packed, so nothing has to be rolled back.
+packed, so nothing has to be rolled back.  The host keeps count of what is packed: a captured
+graph replays one position only, so capture ``HotPath.attention8`` itself where that is wanted.
 """
 BLOCK = 64
 
@@ -32,7 +33,8 @@ class Cache8:
         self.value_scales = torch.zeros_like(self.key_scales)
         self.key_tail = torch.zeros((tail_rows, 4, 256), dtype=torch.float16, device=dev)
         self.value_tail = torch.zeros_like(self.key_tail)
-        self.packed = 0
+        self.packed = 0                  # positions in the packed part
+        self.rows = 0                    # positions that hold a row
 
     def _packed_buffers(self):
         return self.key_codes, self.key_scales, self.value_codes, self.value_scales
@@ -41,6 +43,8 @@ class Cache8:
         """Pack the blocks that are complete before `position`."""
         end = position // BLOCK * BLOCK
         if end > self.packed:
+            if self.hot.capturing():
+                raise RuntimeError('blocks cannot be packed under graph capture: a replay would pack rows that have gone on')
             self.hot.cache8_pack(*self._packed_buffers(), self.key_tail, self.value_tail, self.packed, end)
             self.packed = end
 
@@ -55,11 +59,11 @@ class Cache8:
             at = end % self.key_tail.shape[0]        # whole blocks: the rest does not wrap
             self.key_tail[at:at + rows - end].copy_(key_rows[end:rows])
             self.value_tail[at:at + rows - end].copy_(value_rows[end:rows])
-        self.packed = end
+        self.packed, self.rows = end, rows
 
     def unload(self, key_rows, value_rows, position):
         """Write the first `position` positions as fp16 rows, e.g. to prefill a further block behind them."""
-        if not self.packed <= position <= min(self.packed + self.key_tail.shape[0], key_rows.shape[0], value_rows.shape[0]):
+        if not self.packed <= position <= min(self.rows, key_rows.shape[0], value_rows.shape[0]):
             raise ValueError('position is outside the cache or the given rows')
         import torch
         self.hot.cache8_unpack(key_rows, value_rows, *self._packed_buffers(), 0, self.packed)
@@ -73,6 +77,9 @@ class Cache8:
             raise ValueError(f'position {position} lies in the packed part (up to {self.packed})')
         if position + batch > self.context:
             raise ValueError(f'the cache holds {self.context} positions')
+        if position > self.rows:
+            raise ValueError(f'position {position} leaves a gap: the cache holds {self.rows} rows')
         self.pack(position)
         self.hot.attention8(out, *self._packed_buffers(), self.packed, self.key_tail, self.value_tail, q_gate, key,
                             value, q_norm, k_norm, batch, position, epsilon, workspace)
+        self.rows = position + batch

@@ -106,18 +106,30 @@ class NativeError(RuntimeError):
 # Host-side checks of the 8-bit calls, which take their sizes from the tensors: a wrong shape, element
 # size, layout or device is refused here, before an address reaches a kernel.  They run on every call of
 # a decode step, so they ask a tensor only what is cheap to ask (a CPU tensor's device number is -1).
-def need_tensor(t, itemsize, shape, name, device):
-    if t.shape != shape or t.element_size() != itemsize or t.get_device() != device or device < 0 or not t.is_contiguous():
-        raise ValueError(f'{name} must be a contiguous CUDA tensor of shape {list(shape)} with {itemsize}-byte elements'
-                         + (f' on device {device}' if device >= 0 else ''))
+class ElementTypes:
+    """The element types that the 8-bit calls take; e4m3 codes and workspaces may also be plain bytes."""
+
+    def __init__(self):
+        import torch
+        self.float = (torch.float32,)
+        self.half = (torch.float16,)
+        self.int8 = (torch.int8,)
+        self.e4m3 = (torch.float8_e4m3fn, torch.uint8)
+        self.bytes = (torch.uint8, torch.int8)
 
 
-def need_cache8(key_codes, key_scales, value_codes, value_scales, end, device):
+def need_tensor(t, types, shape, name, device):
+    if t.dtype not in types or t.shape != shape or t.get_device() != device or device < 0 or not t.is_contiguous():
+        raise ValueError(f'{name} must be a contiguous CUDA tensor of shape {list(shape)} and type '
+                         + ' or '.join(str(x) for x in types) + (f' on device {device}' if device >= 0 else ''))
+
+
+def need_cache8(types, key_codes, key_scales, value_codes, value_scales, end, device):
     blocks = key_codes.shape[0]
-    need_tensor(key_codes, 1, (blocks, 4, 64, 256), 'key_codes', device)
-    need_tensor(value_codes, 1, (blocks, 4, 64, 256), 'value_codes', device)
-    need_tensor(key_scales, 4, (blocks, 4), 'key_scales', device)
-    need_tensor(value_scales, 4, (blocks, 4), 'value_scales', device)
+    need_tensor(key_codes, types.int8, (blocks, 4, 64, 256), 'key_codes', device)
+    need_tensor(value_codes, types.int8, (blocks, 4, 64, 256), 'value_codes', device)
+    need_tensor(key_scales, types.float, (blocks, 4), 'key_scales', device)
+    need_tensor(value_scales, types.float, (blocks, 4), 'value_scales', device)
     if end > 64 * blocks:
         raise ValueError(f'the cache holds {blocks} blocks of 64 rows, not {end} rows')
 
@@ -134,6 +146,7 @@ class HotPath:
         self.lib = load_library(library)
         self._workspace = None
         self._workspaces8 = {}
+        self._types = ElementTypes()
 
     # -- helpers ---------------------------------------------------------
     def check(self, code):
@@ -144,6 +157,12 @@ class HotPath:
     def _stream():
         import torch
         return ct.c_void_p(torch.cuda.current_stream().cuda_stream)
+
+    @staticmethod
+    def capturing():
+        """Whether torch's current stream is being captured into a graph."""
+        import torch
+        return torch.cuda.is_current_stream_capturing()
 
     @staticmethod
     def _ptr(t):
@@ -288,15 +307,16 @@ class HotPath:
     def norm8(self, codes, scales, x, weights, residual=None, residual_out=None, normed=None, epsilon=1e-6):
         """qv_norm8: e4m3 codes [tokens][width] and scales [ceil(width/128)][tokens] of the RMSNorm of
         x (+ residual); residual_out and normed, where given, receive the sum and the norm in fp32."""
+        types = self._types
         tokens, width = x.shape
         dev = x.get_device()
-        need_tensor(x, 4, (tokens, width), 'x', dev)
-        need_tensor(codes, 1, (tokens, width), 'codes', dev)
-        need_tensor(scales, 4, (-(-width // 128), tokens), 'scales', dev)
-        need_tensor(weights, 4, (width,), 'weights', dev)
+        need_tensor(x, types.float, (tokens, width), 'x', dev)
+        need_tensor(codes, types.e4m3, (tokens, width), 'codes', dev)
+        need_tensor(scales, types.float, (-(-width // 128), tokens), 'scales', dev)
+        need_tensor(weights, types.float, (width,), 'weights', dev)
         for name, t in (('residual', residual), ('residual_out', residual_out), ('normed', normed)):
             if t is not None:
-                need_tensor(t, 4, (tokens, width), name, dev)
+                need_tensor(t, types.float, (tokens, width), name, dev)
         self._call(dev, self.lib.qv_norm8, codes.data_ptr(), scales.data_ptr(),
                    None if residual_out is None else residual_out.data_ptr(),
                    None if normed is None else normed.data_ptr(), x.data_ptr(),
@@ -304,22 +324,24 @@ class HotPath:
 
     def quantize8(self, codes, scales, x):
         """qv_quantize8: e4m3 codes and scales of x itself."""
+        types = self._types
         tokens, width = x.shape
         dev = x.get_device()
-        need_tensor(x, 4, (tokens, width), 'x', dev)
-        need_tensor(codes, 1, (tokens, width), 'codes', dev)
-        need_tensor(scales, 4, (-(-width // 128), tokens), 'scales', dev)
+        need_tensor(x, types.float, (tokens, width), 'x', dev)
+        need_tensor(codes, types.e4m3, (tokens, width), 'codes', dev)
+        need_tensor(scales, types.float, (-(-width // 128), tokens), 'scales', dev)
         self._call(dev, self.lib.qv_quantize8, codes.data_ptr(), scales.data_ptr(), x.data_ptr(), tokens, width)
 
     def mm8(self, out, weights, weight_scales, codes, scales):
         """qv_mm8: out [tokens][rows] = codes x weights^T, both e4m3 with a scale for every block of 128."""
+        types = self._types
         tokens, width = codes.shape
         rows, blocks, dev = weights.shape[0], -(-width // 128), codes.get_device()
-        need_tensor(codes, 1, (tokens, width), 'codes', dev)
-        need_tensor(scales, 4, (blocks, tokens), 'scales', dev)
-        need_tensor(weights, 1, (rows, width), 'weights', dev)
-        need_tensor(weight_scales, 4, (-(-rows // 128), blocks), 'weight_scales', dev)
-        need_tensor(out, 4, (tokens, rows), 'out', dev)
+        need_tensor(codes, types.e4m3, (tokens, width), 'codes', dev)
+        need_tensor(scales, types.float, (blocks, tokens), 'scales', dev)
+        need_tensor(weights, types.e4m3, (rows, width), 'weights', dev)
+        need_tensor(weight_scales, types.float, (-(-rows // 128), blocks), 'weight_scales', dev)
+        need_tensor(out, types.float, (tokens, rows), 'out', dev)
         self._call(dev, self.lib.qv_mm8, out.data_ptr(), weights.data_ptr(), weight_scales.data_ptr(), codes.data_ptr(),
                    scales.data_ptr(), tokens, width, rows)
 
@@ -339,25 +361,26 @@ class HotPath:
         positions and the fp16 tail.  Without `workspace`, one that is kept for the current stream is used;
         under graph capture it has to be given (attention8_workspace), since the graph goes on using it."""
         import torch
+        types = self._types
         dev, tail = out.get_device(), key_tail.shape[0]
-        need_tensor(out, 4, (batch, 24, 256), 'out', dev)
-        need_tensor(q_gate, 4, (batch, 24, 512), 'q_gate', dev)
-        need_tensor(key, 4, (batch, 4, 256), 'key', dev)
-        need_tensor(value, 4, (batch, 4, 256), 'value', dev)
-        need_tensor(q_norm, 4, (256,), 'q_norm', dev)
-        need_tensor(k_norm, 4, (256,), 'k_norm', dev)
-        need_tensor(key_tail, 2, (tail, 4, 256), 'key_tail', dev)
-        need_tensor(value_tail, 2, (tail, 4, 256), 'value_tail', dev)
-        need_cache8(key_codes, key_scales, value_codes, value_scales, packed, dev)
+        need_tensor(out, types.float, (batch, 24, 256), 'out', dev)
+        need_tensor(q_gate, types.float, (batch, 24, 512), 'q_gate', dev)
+        need_tensor(key, types.float, (batch, 4, 256), 'key', dev)
+        need_tensor(value, types.float, (batch, 4, 256), 'value', dev)
+        need_tensor(q_norm, types.float, (256,), 'q_norm', dev)
+        need_tensor(k_norm, types.float, (256,), 'k_norm', dev)
+        need_tensor(key_tail, types.half, (tail, 4, 256), 'key_tail', dev)
+        need_tensor(value_tail, types.half, (tail, 4, 256), 'value_tail', dev)
+        need_cache8(types, key_codes, key_scales, value_codes, value_scales, packed, dev)
         if workspace is None:
-            if torch.cuda.is_current_stream_capturing():
+            if self.capturing():
                 raise ValueError('attention8 under graph capture needs a workspace of its own (attention8_workspace)')
             which = (dev, torch._C._cuda_getCurrentRawStream(dev))
             workspace = self._workspaces8.get(which)
             if workspace is None:
                 workspace = self._workspaces8[which] = self.attention8_workspace(out.device)
         else:
-            need_tensor(workspace, 1, workspace.shape, 'workspace', dev)
+            need_tensor(workspace, types.bytes, workspace.shape, 'workspace', dev)
         self._call(dev, self.lib.qv_attention8, out.data_ptr(), key_codes.data_ptr(), key_scales.data_ptr(),
                    value_codes.data_ptr(), value_scales.data_ptr(), packed, key_tail.data_ptr(), value_tail.data_ptr(), tail,
                    q_gate.data_ptr(), key.data_ptr(), value.data_ptr(), q_norm.data_ptr(), k_norm.data_ptr(),
@@ -365,19 +388,21 @@ class HotPath:
 
     def cache8_pack(self, key_codes, key_scales, value_codes, value_scales, key_rows, value_rows, begin, end):
         """qv_cache8_pack: positions [begin, end) of fp16 rows (position r at row r % rows) to int8 codes."""
+        types = self._types
         ring, dev = key_rows.shape[0], key_rows.get_device()
-        need_cache8(key_codes, key_scales, value_codes, value_scales, end, dev)
-        need_tensor(key_rows, 2, (ring, 4, 256), 'key_rows', dev)
-        need_tensor(value_rows, 2, (ring, 4, 256), 'value_rows', dev)
+        need_cache8(types, key_codes, key_scales, value_codes, value_scales, end, dev)
+        need_tensor(key_rows, types.half, (ring, 4, 256), 'key_rows', dev)
+        need_tensor(value_rows, types.half, (ring, 4, 256), 'value_rows', dev)
         self._call(dev, self.lib.qv_cache8_pack, key_codes.data_ptr(), key_scales.data_ptr(), value_codes.data_ptr(),
                    value_scales.data_ptr(), key_rows.data_ptr(), value_rows.data_ptr(), begin, end, ring)
 
     def cache8_unpack(self, key_rows, value_rows, key_codes, key_scales, value_codes, value_scales, begin, end, origin=0):
         """qv_cache8_unpack: positions [begin, end) as fp16 rows, position r at row r - origin."""
+        types = self._types
         rows, dev = key_rows.shape[0], key_rows.get_device()
-        need_cache8(key_codes, key_scales, value_codes, value_scales, end, dev)
-        need_tensor(key_rows, 2, (rows, 4, 256), 'key_rows', dev)
-        need_tensor(value_rows, 2, (rows, 4, 256), 'value_rows', dev)
+        need_cache8(types, key_codes, key_scales, value_codes, value_scales, end, dev)
+        need_tensor(key_rows, types.half, (rows, 4, 256), 'key_rows', dev)
+        need_tensor(value_rows, types.half, (rows, 4, 256), 'value_rows', dev)
         if not 0 <= begin - origin <= end - origin <= rows:
             raise ValueError(f'positions [{begin}, {end}) do not fit {rows} rows from position {origin}')
         skip = (begin - origin) * 2048

@@ -43,6 +43,37 @@ def test_cache_object_refuses_what_does_not_fit():
             Cache8(None, context, tail_rows=tail)
 
 
+def test_a_position_behind_a_gap_or_in_the_packed_part_is_refused():
+    from redshift_b200 import Cache8
+    calls = []
+
+    class Recorder:
+        def __getattr__(self, name):
+            return lambda *args: calls.append(name)
+    cache = Cache8(Recorder(), 256, device='cpu:0')
+    step = lambda batch, position: cache.attention(None, None, None, None, None, None, batch, position)  # noqa: E731
+    with pytest.raises(ValueError, match='leaves a gap'):
+        step(1, 1)
+    step(8, 0)
+    step(8, 3)                                           # five of the eight were not kept
+    with pytest.raises(ValueError, match='holds 11 rows'):
+        step(1, 12)
+    for position in range(11, 64):
+        step(1, position)
+    assert 'cache8_pack' not in calls and cache.packed == 0
+    step(8, 64)
+    assert calls.count('cache8_pack') == 1 and cache.packed == 64
+    with pytest.raises(ValueError, match='packed part'):
+        step(1, 63)
+    step(10, 70)
+    for position in range(80, 250):
+        step(1, position)
+    with pytest.raises(ValueError, match='holds 256 positions'):
+        step(10, 250)
+    with pytest.raises(ValueError, match='outside the cache'):
+        cache.unload(cache.key_tail, cache.value_tail, 251)
+
+
 # ------------------------------------------------------------------ the operator
 def _dev(a):
     import torch
@@ -400,4 +431,28 @@ def test_an_attention_layer_in_eight_bits(hot):
         n8 = codes(T, E5)
         hot.norm8(*n8, added, gamma[1], residual=stream, residual_out=stream)
         assert torch.isfinite(stream).all()
+    assert cache.packed == 64 and hot.status() == 0
+
+
+@pytest.mark.gpu
+def test_packing_under_capture_is_refused(hot):
+    """A replay would pack tail rows that hold other positions by then."""
+    import torch
+    from redshift_b200 import Cache8
+    cache = Cache8(hot, 256)
+    q, k, v, qn, kn = _tokens(8, 9200)
+    out = torch.empty((8, 24, 256), device='cuda')
+    for position in range(0, 64, 8):
+        cache.attention(out, q, k, v, qn, kn, 8, position)
+    torch.cuda.synchronize()
+    graph, stream = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        graph.capture_begin()
+        out.zero_()
+        with pytest.raises(RuntimeError, match='capture'):
+            cache.attention(out, q, k, v, qn, kn, 8, 64)
+        graph.capture_end()
+    assert cache.packed == 0 and cache.rows == 64
+    cache.attention(out, q, k, v, qn, kn, 8, 64)
+    torch.cuda.synchronize()
     assert cache.packed == 64 and hot.status() == 0

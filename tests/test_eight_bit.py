@@ -71,6 +71,29 @@ def test_tensors_that_do_not_fit_are_refused():
         hot.cache8_unpack(rows, rows, *cache, 0, 64)
 
 
+@pytest.mark.gpu
+def test_tensors_of_another_type_are_refused(hot):
+    """Types of the same size are not taken for one another."""
+    import torch
+    f = lambda *shape, dtype=torch.float32: torch.zeros(shape, dtype=dtype, device='cuda')  # noqa: E731
+    codes, scales, x = f(2, 128, dtype=torch.uint8), f(1, 2), f(2, 128)
+    for bad in (codes.view(torch.int8), codes.view(torch.float8_e5m2)):
+        with pytest.raises(ValueError, match='codes must be'):
+            hot.quantize8(bad, scales, x)
+        with pytest.raises(ValueError, match='weights must be'):
+            hot.mm8(f(2, 2), bad, f(1, 1), codes, scales)
+    with pytest.raises(ValueError, match='x must be'):
+        hot.norm8(codes, scales, x.to(torch.int32), f(128))
+    cache = [f(1, 4, 64, 256, dtype=torch.int8), f(1, 4), f(1, 4, 64, 256, dtype=torch.int8), f(1, 4)]
+    rows = f(64, 4, 256, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match='key_rows must be'):
+        hot.cache8_pack(*cache, rows, rows, 0, 64)
+    with pytest.raises(ValueError, match='key_codes must be'):
+        hot.cache8_pack(cache[0].view(torch.uint8), *cache[1:], rows.half(), rows.half(), 0, 64)
+    hot.quantize8(codes.view(torch.float8_e4m3fn), scales, x)
+    assert hot.status() == 0
+
+
 # ------------------------------------------------------------------ norm8 / quantize8
 def _dev(a):
     import torch
