@@ -139,8 +139,7 @@ fa_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUten
         }
         QV_STAMP(2);
     };
-    float unused[QR];
-    prepare_queries<false>(p, kv_head, rope, smem + L::SM_P, tmem, q_ready, [&] { issue_early(0, early); }, unused);
+    prepare_queries(p, kv_head, rope, smem + L::SM_P, tmem, q_ready, [&] { issue_early(0, early); });
     if ((warp == 2 || warp == 3) && appends) {
         // The new rows become visible to the TMA loads of this CTA.
         append_rows(p, kv_head, warp - 2, app_lo, app_hi, rope);

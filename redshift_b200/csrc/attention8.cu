@@ -48,7 +48,6 @@
 #include <algorithm>
 #include <stdexcept>
 #include <string>
-#include <type_traits>
 
 namespace qv {
 namespace {
@@ -66,9 +65,9 @@ struct A8Layout {
     static constexpr int SM_KV_STAGE = 2 * TILE_BYTES;
     static constexpr int SM_QSTAGE = EPILOGUE_BYTES;              // the queries on their way to TMEM, then the tail's scratch
     static constexpr int SM_BAR = SM_QSTAGE + 2 * DECODE_ROWS * 256;
-    static constexpr int SM_ROPE = SM_BAR + 384;                  // (cos, sin) [T][32]; then maxima, sums and scales
+    static constexpr int SM_ROPE = SM_BAR + 384;                  // (cos, sin) [T][32]; then maxima and scales
     static constexpr int SMEM_BYTES = SM_ROPE + MAX_DECODE_T * 32 * 8;
-    static_assert((3 * DECODE_ROWS + 2 * MAX_TILES8) * 4 <= MAX_DECODE_T * 32 * 8);
+    static_assert((2 * DECODE_ROWS + 2 * MAX_TILES8) * 4 <= MAX_DECODE_T * 32 * 8);
 };
 static_assert(A8Layout::SMEM_BYTES <= 227 * 1024, "attention kernel exceeds the shared memory of a CTA");
 static_assert(IMAGES * A8Layout::SM_KV_STAGE <= A8Layout::SM_QSTAGE, "the images overlap the staged queries");
@@ -92,30 +91,28 @@ struct Cache8View {
     int ring;                    // rows of the fp16 ring
 };
 
-// Two fp16 numbers of two codes' biased bytes u = code + 128.  Keys: the
-// subnormal numbers u 2^-24; the bias adds 128 times the sum of the query to
-// every score, which the softmax's argument takes off again at no cost.
-// Values: 1024 + u is the fp16 number 0x6400 | u, and its difference to 1152,
-// the code, is exact (a bias of the values would have to be subtracted from
-// sums a thousand times smaller than it).
-constexpr float KEY_UNIT = 0x1p24f;
-template <bool VALUES> __device__ __forceinline__ uint32_t fp16_pair(uint32_t biased, uint32_t select) {
-    if (!VALUES) return __byte_perm(biased, 0u, select);
+// Eight codes as fp16 numbers: 1024 + u is the fp16 number 0x6400 | u of a biased
+// byte u = code + 128, and its difference to 1152, the code, is exact.  (Keys as the
+// subnormal numbers u 2^-24, their bias taken off the scores again, need no
+// subtraction here, 69.7 instead of 72.3 us for 8 tokens at 139,256, but the
+// scores are then small differences of sums four times their size and more, and the
+// outputs' error grew by 1.6.)
+__device__ __forceinline__ uint32_t fp16_pair(uint32_t biased, uint32_t select) {
     const uint32_t w = __byte_perm(biased, 0x64646464u, select);
     return half2_bits(__hsub2(*reinterpret_cast<const __half2 *>(&w), __half2half2(__ushort_as_half(0x6480))));
 }
-template <bool VALUES> __device__ __forceinline__ uint4 fp16_codes(uint32_t a, uint32_t b) {
+__device__ __forceinline__ uint4 fp16_codes(uint32_t a, uint32_t b) {
     a ^= 0x80808080u;
     b ^= 0x80808080u;
-    return make_uint4(fp16_pair<VALUES>(a, 0x4140), fp16_pair<VALUES>(a, 0x4342), fp16_pair<VALUES>(b, 0x4140),
-                      fp16_pair<VALUES>(b, 0x4342));
+    return make_uint4(fp16_pair(a, 0x4140), fp16_pair(a, 0x4342), fp16_pair(b, 0x4140), fp16_pair(b, 0x4342));
 }
 
 // Append (converter warps, positions pos, pos + 8, ... below `end`): RMSNorm +
 // rotary of the new keys, fp16 keys and values into the ring.  What lands in the
-// cache is read by every later token, so the keys are formed in 64 bits and
-// rounded once (in 32 bits a value near a border of two fp16 numbers now and then
-// went to the further one); the warps are idle meanwhile.  Returns the tokens, as
+// cache is read by every later token, so the keys are formed in 64 bits, and the
+// correctly rounded fp32 value goes to fp16 (formed in 32 bits, a value near a border
+// of two fp16 numbers now and then went to the further one); the warps are idle
+// meanwhile.  Returns the tokens, as
 // bits, whose fp16 values are not all finite.
 __device__ __forceinline__ uint32_t append_row8(const FaParams &p, int ring, int kv_head, int pos, int end) {
     const int lane = threadIdx.x & 31;
@@ -152,7 +149,7 @@ __device__ __forceinline__ uint32_t append_row8(const FaParams &p, int ring, int
             __half2 kh[2], vh[2];
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                kh[e] = __halves2half2(__double2half(x[4 * h + 2 * e]), __double2half(x[4 * h + 2 * e + 1]));
+                kh[e] = __floats2half2_rn((float)x[4 * h + 2 * e], (float)x[4 * h + 2 * e + 1]);
                 vh[e] = __floats2half2_rn(v[4 * h + 2 * e], v[4 * h + 2 * e + 1]);
                 const float2 f = __half22float2(__habs2(vh[e]));
                 finite = finite && f.x <= 65504.f && f.y <= 65504.f;
@@ -241,16 +238,15 @@ __global__ void __launch_bounds__(THREADS8, 1) attention8_kernel(const FaParams 
 #pragma unroll
             for (int i = 0; i < 8; ++i) x[i] = ld_once(reinterpret_cast<const uint4 *>(src + i * 2 * HD));
         };
-        auto convert = [&](auto values, uint8_t *dst) {
-            constexpr bool V = decltype(values)::value;
+        auto convert = [&](uint8_t *dst) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 uint8_t *d = dst + image + i * 256;
                 const int swizzle = (2 * i + odd) & 7;
                 *reinterpret_cast<uint4 *>(d + (((2 * q) ^ swizzle) << 4)) =
-                    fp16_codes<V>(x[i].x, x[i].y);
+                    fp16_codes(x[i].x, x[i].y);
                 *reinterpret_cast<uint4 *>(d + (((2 * q + 1) ^ swizzle) << 4)) =
-                    fp16_codes<V>(x[i].z, x[i].w);
+                    fp16_codes(x[i].z, x[i].w);
             }
         };
         // A tile of fp16 rows; rows past the last position and value rows in `skip` (new tokens, bits) are zero.
@@ -296,8 +292,7 @@ __global__ void __launch_bounds__(THREADS8, 1) attention8_kernel(const FaParams 
             if (fresh && !warp_wait(app_done, 0, abort_flag)) break;
             if (j >= 2 && !warp_wait(empty + s, (uint32_t)((j >> 1) - 1) & 1, abort_flag)) break;
             if (j >= code_tiles) copy_rows(dst, rows, j, part && fresh ? *reinterpret_cast<volatile uint32_t *>(bad_values) : 0u);
-            else if (part) convert(std::true_type{}, dst);
-            else convert(std::false_type{}, dst);
+            else convert(dst);
             if (j + 1 < code_tiles) load(j + 1);
             publish(full + s);
         }
@@ -352,8 +347,7 @@ __global__ void __launch_bounds__(THREADS8, 1) attention8_kernel(const FaParams 
         k_scale = c.ks[(size_t)(tile0 + threadIdx.x) * NKV + kv_head];
         v_scale = c.vs[(size_t)(tile0 + threadIdx.x) * NKV + kv_head];
     }
-    float row_sums[QR];
-    prepare_queries<true>(p, kv_head, rope, smem + L::SM_QSTAGE, tmem, q_ready, [&] { mbar_arrive(q_loaded); }, row_sums);
+    prepare_queries(p, kv_head, rope, smem + L::SM_QSTAGE, tmem, q_ready, [&] { mbar_arrive(q_loaded); });
     {
         // ------------------------------------------------ softmax
         // Lanes 32g + i and 32g + 16 + i of TMEM hold the hi and lo halves of query
@@ -367,24 +361,18 @@ __global__ void __launch_bounds__(THREADS8, 1) attention8_kernel(const FaParams 
         float m_use[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 #pragma unroll
         for (int u = 0; u < 2; ++u) last[u] = r0 + 8 * u < rows ? p.position + (r0 + 8 * u) / GROUP : -1;
-        // Once the queries are rotated, the rotary table's place takes the queries'
-        // sums (row warp + 8 j), the scales and the running maxima.
+        // Once the queries are rotated, the rotary table's place takes the running
+        // maxima and the scales.
         float *maxima = reinterpret_cast<float *>(rope);           // [tile parity][64 rows]
-        float *sums = maxima + 2 * DECODE_ROWS, *scales = sums + DECODE_ROWS, bias[2];
+        float *scales = maxima + 2 * DECODE_ROWS;
         named_barrier(4, 32 * SOFT_WARPS);
         if (threadIdx.x < MAX_TILES8) *reinterpret_cast<float2 *>(scales + 2 * threadIdx.x) = make_float2(k_scale, v_scale);
-        if (lane == 0)
-#pragma unroll
-            for (int i = 0; i < QR; ++i) sums[warp + 8 * i] = row_sums[i];
         named_barrier(6, 32 * SOFT_WARPS);
-#pragma unroll
-        for (int u = 0; u < 2; ++u) bias[u] = 128.f * sums[r0 + 8 * u];
         for (int j = turn; j < ntiles; j += 2) {
             const int b = turn;
-            // a score in log2 units: x to_log2 + unbias
             const bool codes = j < code_tiles;
             const float2 scale = *reinterpret_cast<const float2 *>(scales + 2 * j);
-            const float score_log2 = SCORE_LOG2 * scale.x, to_log2 = codes ? score_log2 * KEY_UNIT : score_log2;
+            const float to_log2 = SCORE_LOG2 * scale.x;            // a score in log2 units (rows have the scales 1)
             // a scale of (almost) zero: its codes count nothing, its keys still do; NaN stays
             const float vs = scale.y < 0x1p-100f ? 0x1p-100f : scale.y;
             const float v_log2 = log2_approx(vs), v_inv = rcp_approx(vs);
@@ -433,7 +421,7 @@ __global__ void __launch_bounds__(THREADS8, 1) attention8_kernel(const FaParams 
             // The largest of this thread's columns, in log2 units.  The running maximum
             // moves only when a tile's is far above it, so that most tiles need no
             // more than this and a vote.
-            float m[2], unbias[2];
+            float m[2];
             bool above = false;
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
@@ -443,8 +431,7 @@ __global__ void __launch_bounds__(THREADS8, 1) attention8_kernel(const FaParams 
                     m0 = fmaxf(m0, fmaxf(x[2 * n + u].x, x[2 * n + u].y));
                     m1 = fmaxf(m1, fmaxf(x[2 * n + 2 + u].x, x[2 * n + 2 + u].y));
                 }
-                unbias[u] = codes ? -bias[u] * score_log2 : 0.f;
-                m[u] = fmaf(fmaxf(m0, m1), to_log2, unbias[u] + v_log2);       // -inf stays -inf
+                m[u] = fmaf(fmaxf(m0, m1), to_log2, v_log2);       // -inf stays -inf
                 above = above || m[u] > before[u] + RESCALE_THRESHOLD;
             }
             const bool need = __any_sync(0xffffffffu, above);
@@ -494,7 +481,7 @@ __global__ void __launch_bounds__(THREADS8, 1) attention8_kernel(const FaParams 
                     l[u] *= exp2_approx(m_use[u] - m[u]);
                     m_use[u] = m[u];
                 }
-                const float f = unbias[u] + v_log2 + P_BIAS - (m_use[u] == -INFINITY ? 0.f : m_use[u]);
+                const float f = v_log2 + P_BIAS - (m_use[u] == -INFINITY ? 0.f : m_use[u]);
                 shift[u] = make_float2(f, f);
                 sum[u] = make_float2(0.f, 0.f);
             }
@@ -523,7 +510,7 @@ __global__ void __launch_bounds__(THREADS8, 1) attention8_kernel(const FaParams 
         }
         // The rows' maximum and sum, for the split combine: the last tile's warp has
         // the final maximum, the other brings its sum to it.
-        float *finals = maxima + 2 * DECODE_ROWS;                  // (max, sum) [64], over the queries' sums and the scales
+        float *finals = maxima + 2 * DECODE_ROWS;                  // (max, sum) [64], over the scales
         const bool ends = turn == ((ntiles - 1) & 1);
         named_barrier(4, 32 * SOFT_WARPS);
 #pragma unroll

@@ -420,13 +420,11 @@ static __device__ void decode_tail(const FaParams &p, int g, uint8_t *scratch, f
 // loaded, normalised, rotated and placed in TMEM as the A operand of the QK
 // MMA.  Thread 0 calls `rows_arrived` once every warp's rows have arrived;
 // `qstage` is 32 KB of shared memory that is idle until the first softmax (128
-// A rows x 256 bytes); every warp arrives on q_ready at the end.  SUMS:
-// row_sums[j] becomes the sum of the warp's prepared row warp + 8 j.
+// A rows x 256 bytes); every warp arrives on q_ready at the end.
 constexpr int QR = DECODE_ROWS / 8;              // query rows of a warp
-template <bool SUMS, class F>
+template <class F>
 __device__ __forceinline__ void prepare_queries(const FaParams &p, int kv_head, float2 *rope, uint8_t *qstage,
-                                                uint32_t tmem, uint64_t *q_ready, F &&rows_arrived,
-                                                float (&row_sums)[QR]) {
+                                                uint32_t tmem, uint64_t *q_ready, F &&rows_arrived) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     float4 xa[QR], xb[QR], n0, n1;
     {
@@ -491,7 +489,6 @@ __device__ __forceinline__ void prepare_queries(const FaParams &p, int kv_head, 
         split(x0[2], x0[3], hw[j][0][1], hw[j][0][3]);
         split(x1[0], x1[1], hw[j][1][0], hw[j][1][2]);
         split(x1[2], x1[3], hw[j][1][1], hw[j][1][3]);
-        if (SUMS) row_sums[j] = warp_sum((x0[0] + x0[1]) + (x0[2] + x0[3]) + (x1[0] + x1[1]) + (x1[2] + x1[3]));
     }
     const int sub = (lane & 1) * 8;
     const int arow = (warp & 3) * 32 + lane, col_half = warp >> 2;

