@@ -101,9 +101,9 @@ template <int NT> struct Few {
     static constexpr int SLOT_FLOATS = NT + 4;
     static constexpr int SM_SCALE = STAGES * STAGE;
     static constexpr int SM_BAR = SM_SCALE + SLOTS * SLOT_FLOATS * 4;
-    static constexpr int SMEM = SM_BAR + 256;
+    static constexpr int SMEM = SM_BAR + 384;
     static_assert(NT * ROWS * 4 <= STAGES * STAGE, "partial sums exceed the ring");
-    static_assert((2 * STAGES + 2 * BUFS + SLOTS + 1) * 8 + 8 <= 256, "barrier area");
+    static_assert((2 * STAGES + 2 * BUFS + 2 * SLOTS + 1) * 8 + 8 <= 384, "barrier area");
 };
 
 template <int NT>
@@ -113,7 +113,7 @@ few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUte
     extern __shared__ __align__(1024) uint8_t smem[];
     uint64_t *full = reinterpret_cast<uint64_t *>(smem + L::SM_BAR), *empty = full + L::STAGES;
     uint64_t *d_full = empty + L::STAGES, *d_empty = d_full + L::BUFS, *s_full = d_empty + L::BUFS;
-    uint64_t *mma_done = s_full + L::SLOTS;
+    uint64_t *s_empty = s_full + L::SLOTS, *mma_done = s_empty + L::SLOTS;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(mma_done + 1);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
     float *slots = reinterpret_cast<float *>(smem + L::SM_SCALE);
@@ -127,7 +127,7 @@ few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUte
     if (threadIdx.x == 0) {
         for (int i = 0; i < L::STAGES; ++i) { mbar_init(full + i, 1); mbar_init(empty + i, 1); }
         for (int i = 0; i < L::BUFS; ++i) { mbar_init(d_full + i, 1); mbar_init(d_empty + i, L::SUM_WARPS); }
-        for (int i = 0; i < L::SLOTS; ++i) mbar_init(s_full + i, 32);
+        for (int i = 0; i < L::SLOTS; ++i) { mbar_init(s_full + i, 32); mbar_init(s_empty + i, L::SUM_WARPS); }
         mbar_init(mma_done, 1);
         *abort_flag = bad_base ? 1 : 0;
         if (bad_base) raise_status(STATUS_BAD_ARGUMENT);
@@ -181,10 +181,10 @@ few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUte
             live[i] = t < NT && t0 + t < p.tokens;
             src[i] = p.scales + (size_t)b0 * p.tokens + (live[i] ? t0 + t : 0);
         }
-        for (int j = 0, s = 0, lap = 0, slot = 0; j < n; ++j) {
-            // A slot is free with its stage: the MMA of block j - STAGES has run,
-            // which waited until block j - SLOTS had left its accumulator.
-            if (lap > 0 && !warp_wait8(empty + s, (lap - 1) & 1, abort_flag)) { ok = false; break; }
+        for (int j = 0, slot = 0, lap = 0; j < n; ++j) {
+            // A slot has barriers of its own: `empty` may go on by two phases while
+            // this warp is late, and its parity would then seem not to have changed.
+            if (lap > 0 && !warp_wait8(s_empty + slot, (lap - 1) & 1, abort_flag)) { ok = false; break; }
             float *d = slots + slot * L::SLOT_FLOATS;
 #pragma unroll
             for (int i = 0; i < PER_LANE; ++i) {
@@ -193,8 +193,7 @@ few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUte
             }
             if (lane == 0) copy_float(d + NT, w_src + j, true);
             arrive_copies(s_full + slot);
-            if (++s == L::STAGES) { s = 0; ++lap; }
-            if (++slot == L::SLOTS) slot = 0;
+            if (++slot == L::SLOTS) { slot = 0; ++lap; }
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
     } else if (warp == 1) {
@@ -243,7 +242,7 @@ few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUte
             }
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(d_empty + d);
+            if (lane == 0) { mbar_arrive(d_empty + d); mbar_arrive(s_empty + slot); }
         }
     }
     __syncwarp();
@@ -316,14 +315,14 @@ few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUte
 // cycles a block.
 struct Many {
     static constexpr int MT = 128, NT = 256;                 // tokens, weight rows of a tile
-    static constexpr int STAGES = 4, BUFS = 2, SLOTS = STAGES + BUFS, SCALE_WARP = 10, THREADS = 352;
+    static constexpr int STAGES = 4, BUFS = 2, SLOTS = STAGES + BUFS, SUM_WARPS = 8, SCALE_WARP = 10, THREADS = 352;
     static constexpr int X_BYTES = MT * KB, W_BYTES = NT * KB, STAGE = X_BYTES + W_BYTES;
     static constexpr int SLOT_FLOATS = MT + 4;
     static constexpr int OUT_ROW = 20;                       // floats of a staged row: 16 columns and a pad
     static constexpr int SM_OUT = STAGES * STAGE;            // [8 warps][32 rows][OUT_ROW]
     static constexpr int SM_SCALE = SM_OUT + 8 * 32 * OUT_ROW * 4;
     static constexpr int SM_BAR = SM_SCALE + SLOTS * SLOT_FLOATS * 4;
-    static constexpr int SMEM = SM_BAR + 256;
+    static constexpr int SMEM = SM_BAR + 384;
     static_assert(SMEM <= 227 * 1024, "shared memory of a CTA");
 };
 
@@ -333,7 +332,7 @@ many_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUt
     extern __shared__ __align__(1024) uint8_t smem[];
     uint64_t *full = reinterpret_cast<uint64_t *>(smem + L::SM_BAR), *empty = full + L::STAGES;
     uint64_t *d_full = empty + L::STAGES, *d_empty = d_full + L::BUFS, *s_full = d_empty + L::BUFS;
-    uint64_t *mma_done = s_full + L::SLOTS;
+    uint64_t *s_empty = s_full + L::SLOTS, *mma_done = s_empty + L::SLOTS;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(mma_done + 1);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
     float *slots = reinterpret_cast<float *>(smem + L::SM_SCALE);
@@ -342,8 +341,8 @@ many_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUt
     const bool bad_base = (smem_addr(smem) & 1023) != 0;
     if (threadIdx.x == 0) {
         for (int i = 0; i < L::STAGES; ++i) { mbar_init(full + i, 1); mbar_init(empty + i, 1); }
-        for (int i = 0; i < L::BUFS; ++i) { mbar_init(d_full + i, 1); mbar_init(d_empty + i, 8); }
-        for (int i = 0; i < L::SLOTS; ++i) mbar_init(s_full + i, 32);
+        for (int i = 0; i < L::BUFS; ++i) { mbar_init(d_full + i, 1); mbar_init(d_empty + i, L::SUM_WARPS); }
+        for (int i = 0; i < L::SLOTS; ++i) { mbar_init(s_full + i, 32); mbar_init(s_empty + i, L::SUM_WARPS); }
         mbar_init(mma_done, 1);
         *abort_flag = bad_base ? 1 : 0;
         if (bad_base) raise_status(STATUS_BAD_ARGUMENT);
@@ -391,7 +390,7 @@ many_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUt
         }
     } else if (warp == L::SCALE_WARP) {
         // ------------------------------------------------ scales, by small copies
-        int s = 0, lap = 0, slot = 0;
+        int slot = 0, lap = 0;
         bool ok = true;
         for (int i = 0; i < mine && ok; ++i) {
             const int tile = blockIdx.x + i * gridDim.x, m0 = tile % p.m_tiles * L::MT, n0 = tile / p.m_tiles * L::NT;
@@ -405,9 +404,7 @@ many_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUt
             const bool w_live = n0 / ROWS + lane < row_blocks;
             const float *w_src = p.weight_scales + (size_t)(w_live ? n0 / ROWS + lane : 0) * p.blocks;
             for (int b = 0; b < p.blocks; ++b) {
-                // A slot is free with its stage: the MMA of the block STAGES before has
-                // run, which waited until the block SLOTS before had left TMEM.
-                if (lap > 0 && !warp_wait8(empty + s, (lap - 1) & 1, abort_flag)) { ok = false; break; }
+                if (lap > 0 && !warp_wait8(s_empty + slot, (lap - 1) & 1, abort_flag)) { ok = false; break; }
                 float *d = slots + slot * L::SLOT_FLOATS;
 #pragma unroll
                 for (int t = 0; t < 4; ++t) {
@@ -416,8 +413,7 @@ many_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUt
                 }
                 if (lane < 2) copy_float(d + L::MT + lane, w_src + b, w_live);
                 arrive_copies(s_full + slot);
-                if (++s == L::STAGES) { s = 0; ++lap; }
-                if (++slot == L::SLOTS) slot = 0;
+                if (++slot == L::SLOTS) { slot = 0; ++lap; }
             }
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
@@ -477,7 +473,7 @@ many_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUt
                 }
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(d_empty + d);
+                if (lane == 0) { mbar_arrive(d_empty + d); mbar_arrive(s_empty + slot); }
             }
             if (!ok) break;
             // 16 columns at a time through shared memory: 64-byte pieces of eight rows per store.
