@@ -310,7 +310,8 @@ int qv_attention_noalloc(float *out, void *key_cache, void *value_cache,
  * (no counterpart in the reference).  Device memory, asynchronous on
  * `stream`, nothing is allocated.  Together they run an attention layer:
  * qv_norm8 -> qv_mm8 (q and gate, k, v) -> qv_attention8 (with
- * qv_cache8_pack every 64 tokens) -> qv_quantize8 -> qv_mm8.
+ * qv_cache8_pack every 64 tokens) -> qv_quantize8 -> qv_mm8.  fp32 buffers
+ * are 4-byte aligned.
  *
  * e4m3 codes: [tokens][width] bytes with fp32 scales
  * [ceil(width/128)][tokens]; a value is code * scale, where a scale belongs
@@ -375,7 +376,8 @@ int qv_cache8_unpack(void *key_rows, void *value_rows, const void *key_codes,
  * `workspace`: qv_attention8_workspace(batch, position) bytes (0 = invalid
  * arguments), 256-byte aligned, zero-filled once before its first use; it
  * serves one call at a time, so graphs that may run at the same time need one
- * each. */
+ * each.  As with qv_attention, the CTAs of a launch wait for one another: on
+ * streams that run side by side, keep the attention calls on one priority. */
 size_t qv_attention8_workspace(int batch, int position);
 int qv_attention8(float *out, const void *key_codes, const float *key_scales,
                   const void *value_codes, const float *value_scales, int packed,

@@ -237,15 +237,22 @@ __device__ __forceinline__ void store_codes(const Norm8Params &p, int token, int
 // meets in shared memory, and a block's maximum is a reduction inside one warp.
 // 4,096 rows x 5,120 with a residual: 45 us (272 MB, 6.0 TB/s); one row 3.6 us.
 constexpr int PER_WARP = 5, MAX_WARPS = 28;   // 140 blocks: 17,920 columns
+// The row's sum of all lanes' values (`red`: one float of each warp).
+__device__ __forceinline__ float row_sum(float *red, float v, int warp, int lane, int warps) {
+    const float s = warp_sum(v);
+    if (lane == 0) red[warp] = s;
+    __syncthreads();
+    return warp_sum(lane < warps ? red[lane] : 0.f);
+}
 template <bool VEC>
 __global__ void __launch_bounds__(32 * MAX_WARPS) norm8_kernel(const Norm8Params p) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
     const int token = blockIdx.x;
     const size_t row = (size_t)token * p.width;
-    __shared__ float red[32];
+    __shared__ float red[2][32];
     grid_dependency_wait();
     if (threadIdx.x == 0) launch_dependents();
-    float v[PER_WARP][4], w[PER_WARP][4], ss[PER_WARP];
+    float v[PER_WARP][4], w[PER_WARP][4];
 #pragma unroll
     for (int i = 0; i < PER_WARP; ++i) load_columns<VEC>(p.x + row, (warp + i * warps) * 128 + 4 * lane, p.width, v[i]);
     if (p.residual) {
@@ -260,14 +267,20 @@ __global__ void __launch_bounds__(32 * MAX_WARPS) norm8_kernel(const Norm8Params
     }
 #pragma unroll
     for (int i = 0; i < PER_WARP; ++i) load_columns<VEC>(p.weights, (warp + i * warps) * 128 + 4 * lane, p.width, w[i]);
+    auto squares = [&](float f) {                 // of this lane's columns times f
+        float ss[PER_WARP];
 #pragma unroll
-    for (int i = 0; i < PER_WARP; ++i)
-        ss[i] = (v[i][0] * v[i][0] + v[i][1] * v[i][1]) + (v[i][2] * v[i][2] + v[i][3] * v[i][3]);
-    const float s = warp_sum((ss[0] + ss[1]) + (ss[2] + ss[3]) + ss[4]);
-    if (lane == 0) red[warp] = s;
-    __syncthreads();
-    const float all = warp_sum(lane < warps ? red[lane] : 0.f);
-    const float inv = __frsqrt_rn(__fdiv_rn(all, (float)p.width) + p.eps);
+        for (int i = 0; i < PER_WARP; ++i) {
+            const float a = v[i][0] * f, b = v[i][1] * f, c = v[i][2] * f, d = v[i][3] * f;
+            ss[i] = (a * a + b * b) + (c * c + d * d);
+        }
+        return (ss[0] + ss[1]) + (ss[2] + ss[3]) + ss[4];
+    };
+    float all = row_sum(red[0], squares(1.f), warp, lane, warps), inv = __frsqrt_rn(__fdiv_rn(all, (float)p.width) + p.eps);
+    if (all > 0x1p126f) {                         // squares beyond fp32: those of the row times 2^-64
+        all = row_sum(red[1], squares(0x1p-64f), warp, lane, warps);
+        inv = __frsqrt_rn(__fdiv_rn(all, (float)p.width)) * 0x1p-64f;
+    }
 #pragma unroll
     for (int i = 0; i < PER_WARP; ++i) {
         const int block = warp + i * warps, c = block * 128 + 4 * lane;

@@ -88,6 +88,9 @@ void check_delta_dims(int key_heads, int value_heads, int dim) {
             value_heads <= 48 && value_heads % key_heads == 0, "unsupported DeltaNet dimensions");
 }
 bool aligned16(const void *a) { return (reinterpret_cast<uintptr_t>(a) & 15) == 0; }
+template <class... T> void check_floats(const T *...a) {
+    require(((reinterpret_cast<uintptr_t>(a) % sizeof(float) == 0) && ...), "fp32 buffers must be 4-byte aligned");
+}
 cudaStream_t as_stream(void *s) { return static_cast<cudaStream_t>(s); }
 
 // ------------------------------------------------------------------ attention
@@ -555,6 +558,7 @@ int qv_cache8_pack(void *key_codes, float *key_scales, void *value_codes, float 
         require(key_codes && key_scales && value_codes && value_scales && key_rows && value_rows, "null cache buffer");
         require(aligned16(key_codes) && aligned16(value_codes) && aligned16(key_rows) && aligned16(value_rows),
                 "cache codes and rows must be 16-byte aligned");
+        check_floats(key_scales, value_scales);
         qv::cache8_pack(static_cast<int8_t *>(key_codes), key_scales, static_cast<int8_t *>(value_codes), value_scales,
                         static_cast<const __half *>(key_rows), static_cast<const __half *>(value_rows), begin, end,
                         ring_rows, as_stream(stream));
@@ -568,6 +572,7 @@ int qv_cache8_unpack(void *key_rows, void *value_rows, const void *key_codes, co
         require(key_codes && key_scales && value_codes && value_scales && key_rows && value_rows, "null cache buffer");
         require(aligned16(key_codes) && aligned16(value_codes) && aligned16(key_rows) && aligned16(value_rows),
                 "cache codes and rows must be 16-byte aligned");
+        check_floats(key_scales, value_scales);
         qv::cache8_unpack(static_cast<__half *>(key_rows), static_cast<__half *>(value_rows),
                           static_cast<const int8_t *>(key_codes), key_scales, static_cast<const int8_t *>(value_codes),
                           value_scales, begin, end, as_stream(stream));
@@ -596,6 +601,7 @@ int qv_attention8(float *out, const void *key_codes, const float *key_scales, co
                 aligned16(q_gate) && aligned16(key) && aligned16(value) && aligned16(q_norm) && aligned16(k_norm),
                 "attention buffers must be 16-byte aligned");
         require((reinterpret_cast<uintptr_t>(workspace) & 255) == 0, "the workspace must be 256-byte aligned");
+        check_floats(out, key_scales, value_scales);
         qv::attention8_run(out, static_cast<const int8_t *>(key_codes), key_scales, static_cast<const int8_t *>(value_codes),
                            value_scales, packed, static_cast<__half *>(key_tail), static_cast<__half *>(value_tail),
                            tail_rows, q_gate, key, value, q_norm, k_norm, batch, position, epsilon, workspace,
@@ -609,6 +615,7 @@ int qv_norm8(void *codes, float *scales, float *residual_out, float *normed, con
         require(tokens >= 1 && tokens <= kMaxContext, "tokens must be between 1 and 139264");
         check_epsilon(epsilon);
         require(codes && scales && x && weights, "null normalization buffer");
+        check_floats(scales, residual_out, normed, x, residual, weights);
         require(!residual_out || residual_out != normed, "residual_out and normed must not share a buffer");
         require(width > 0 && width <= 17408, "invalid normalization width");
         qv::norm8(static_cast<uint8_t *>(codes), scales, residual_out, normed, x, residual, weights, tokens, width,
@@ -620,6 +627,7 @@ int qv_quantize8(void *codes, float *scales, const float *x, int tokens, int wid
     return guarded([&] {
         require(tokens >= 1 && tokens <= kMaxContext, "tokens must be between 1 and 139264");
         require(codes && scales && x, "null quantization buffer");
+        check_floats(scales, x);
         require(width > 0 && width <= 17408, "invalid quantization width");
         qv::norm8(static_cast<uint8_t *>(codes), scales, nullptr, nullptr, x, nullptr, nullptr, tokens, width, 1.f,
                   as_stream(stream));
@@ -634,6 +642,7 @@ int qv_mm8(float *out, const void *weights, const float *weight_scales, const vo
         require(width >= 16 && width <= 65536 && width % 16 == 0 && rows > 0 && rows <= 248320,
                 "invalid projection dimensions");
         require(aligned16(weights) && aligned16(codes), "e4m3 codes must be 16-byte aligned");
+        check_floats(out, weight_scales, scales);
         qv::mm8(out, weights, weight_scales, codes, scales, tokens, width, rows, as_stream(stream));
     });
 }

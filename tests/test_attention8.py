@@ -32,6 +32,9 @@ def test_rejects_invalid_arguments_before_accessing_buffers(lib):
     for name in ('kc', 'vc', 'kt', 'vt', 'q_gate', 'key', 'value', 'q_norm', 'k_norm', 'ws'):
         assert _call(lib, **{name: ct.c_void_p(4104)}) == -1
         assert b'aligned' in lib.qv_error()
+    for name in ('out', 'ks', 'vs'):
+        assert _call(lib, **{name: ct.c_void_p(4098)}) == -1
+        assert lib.qv_error() == b'fp32 buffers must be 4-byte aligned'
     assert lib.qv_attention8_workspace(0, 5) == 0 and lib.qv_attention8_workspace(11, 5) == 0
     assert lib.qv_attention8_workspace(1, 139264) == 0 and lib.qv_attention8_workspace(10, 139254) > 0
 

@@ -47,6 +47,18 @@ def test_rejects_invalid_arguments_before_accessing_buffers(lib):
     for begin, end in ((-1, 5), (6, 5), (0, 139265)):
         assert lib.qv_cache8_unpack(v, v, v, v, v, v, begin, end, None) == -1
     assert lib.qv_cache8_unpack(v, None, v, v, v, v, 0, 5, None) == -1
+    off = ct.c_void_p(4098)                               # no fp32 buffer starts there
+    for i in range(1, 7):
+        assert lib.qv_norm8(*[off if k == i else ct.c_void_p(4096 + 65536 * k) for k in range(7)], 1, 128, 1e-6, None) == -1
+        assert b'4-byte aligned' in lib.qv_error()
+    for i in (1, 2):
+        assert lib.qv_quantize8(*[off if k == i else v for k in range(3)], 1, 128, None) == -1
+    for i in (0, 2, 4):
+        assert lib.qv_mm8(*[off if k == i else v for k in range(5)], 1, 128, 1, None) == -1
+        assert b'4-byte aligned' in lib.qv_error()
+    for i in (1, 3):
+        assert lib.qv_cache8_pack(*[off if k == i else v for k in range(6)], 0, 64, 64, None) == -1
+        assert lib.qv_cache8_unpack(*[off if k == i + 2 else v for k in range(6)], 0, 64, None) == -1
     # an empty range is no work, and no error
     assert lib.qv_cache8_pack(v, v, v, v, v, v, 64, 64, 128, None) == 0
     assert lib.qv_cache8_unpack(v, v, v, v, v, v, 5, 5, None) == 0
@@ -151,6 +163,31 @@ def test_norm8_matches_its_definition(hot, tokens, width, form):
     slack = _norm_slack(width)
     assert (np.abs(normed.cpu().numpy() - y) <= slack * np.abs(y) + 2.0 ** -140).all()
     _check_codes(y, codes.cpu().numpy(), scales.cpu().numpy(), slack)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('exponent', [-60, 55, 63, 64, 90, 118])
+def test_norm8_of_rows_whose_squares_leave_fp32(hot, exponent):
+    """Rows whose squares underflow or overflow; a value of infinity makes its block NaN and the others zero."""
+    import torch
+    rng = np.random.default_rng(7150 + exponent)
+    x = np.ldexp(rng.standard_normal((5, 900)), exponent).astype(np.float32)
+    x[1, 300:] *= np.float32(2.0 ** -80)
+    x[4, 200] = np.inf
+    w = (1 + 0.3 * rng.standard_normal(900)).astype(np.float32)
+    codes = torch.full((5, 900), 0x55, dtype=torch.uint8, device='cuda')
+    scales, normed, out = torch.zeros((8, 5), device='cuda'), torch.empty((5, 900), device='cuda'), torch.empty((5, 900), device='cuda')
+    hot.norm8(codes, scales, _dev(x), _dev(w), residual_out=out, normed=normed)
+    torch.cuda.synchronize()
+    assert np.array_equal(out.cpu().numpy(), x)
+    y = E.norm(x[:4], w)[1]
+    slack = _norm_slack(900)
+    keep = np.abs(y) > 2.0 ** -100                     # a product below fp32's normal range has fewer bits
+    assert (np.abs(normed.cpu().numpy()[:4] - y)[keep] <= slack * np.abs(y)[keep]).all()
+    s = scales.cpu().numpy()
+    assert np.isnan(s[1, 4]) and not np.delete(s[:, 4], 1).any() and not codes.cpu().numpy()[4].any()
+    rows = [0, 2, 3]
+    _check_codes(y[rows], codes.cpu().numpy()[rows], s[:, rows], slack)
 
 
 @pytest.mark.gpu
