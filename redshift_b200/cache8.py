@@ -1,6 +1,6 @@
 """An attention layer's K/V cache in 8 bits, as a decode loop keeps it.
 
-``Cache8`` owns the buffers of ``qv_attention8`` for one layer (2,056 bytes a position instead of
+``Cache8`` owns the buffers of ``qv_attention8`` for one layer (2,048.5 bytes a position instead of
 4,096, and a tail of fp16 rows) and packs the tail's oldest block whenever it is complete::
 
     cache = Cache8(hot, context=32768)

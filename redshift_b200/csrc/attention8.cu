@@ -10,14 +10,14 @@
 // tile of 64 positions is one block, so its two scales are one factor of its
 // scores and one of its probabilities.
 //
-// The floor is the cache's bytes, 2 KB a position: 8 tokens at 139,256 take 71 us
-// (4.0 TB/s, 390 TFLOP/s of products, 44 us at the copy rate), 5 at 32,767 28 us, 1
+// The floor is the cache's bytes, 2 KB a position: 8 tokens at 139,256 take 73 us
+// (3.9 TB/s, 375 TFLOP/s of products, 44 us at the copy rate), 5 at 32,767 28 us, 1
 // at 777 12 us; the fp16 cache's kernel takes 101 us for the longest.  What bounds
 // it is what a tile moves through shared memory (fp16 images written 64 KB and
-// read 64 KB by the MMAs, codes 32 KB: half as much again when the codes were
-// staged there too, 73 us) and, in calls without a pause, the power limit: 990 W
-// and 1.5 GHz, 86 us.  About 12 us of a call are its two ends: 4 us to the first
-// tile, 8 us from the last one through the splits' combination.
+// read 64 KB by the MMAs, codes 32 KB: half as much again, and 3 % slower, when the
+// codes were staged there too) and, in calls without a pause, the power limit: 990 W
+// and 1.45 GHz, 88 us.  About 10 us of a call are its two ends: 4.4 us to the first
+// scores, 5.5 us from the last product through the splits' combination.
 // What keeps the tensor cores fed at twice the fp16 cache's tile rate:
 //  * eight converter warps (four for K, four for V) write the codes as exact fp16
 //    numbers into the MMA's swizzled operand images.  They ask for the next tile's

@@ -18,8 +18,8 @@
 //  * many_kernel (128 tokens as the MMA's M, 256 weight rows as its N): persistent
 //    CTAs.  With tokens in the TMEM lanes the two scales of a thread's columns are
 //    one factor per block.  Bound by the way of a block's sums out of TMEM, see
-//    there (4,001 x 5,120 x 17,408: 390 us, 1.8 PFLOP/s; in calls without a pause the
-//    power limit holds the SMs at 1.5 GHz, 455 us).
+//    there (4,001 x 5,120 x 17,408: 368-410 us, up to 1.9 PFLOP/s; in calls without a
+//    pause the power limit holds the SMs at 1.3-1.5 GHz, 425-455 us).
 #include "common.cuh"
 #include "hotpath.h"
 
@@ -305,9 +305,9 @@ few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUte
 
 // ---------------------------------------------------------------- many tokens
 // A block's MMAs take 513 cycles, scaling and adding its 128 x 256 sums 256 cycles of
-// every FMA lane, and TMEM holds the sums of two blocks.  A block takes about 900
-// cycles: its sums' way from the MMA through two barriers and back, halved, and the
-// output of a tile, which waits for the stores.  Measured and not faster (4,001 x 5,120
+// every FMA lane, and TMEM holds the sums of two blocks.  A block takes 800 cycles:
+// its sums' way from the MMA through two barriers and back, halved; the output of a
+// tile, which waits for the stores, takes 7,000.  Measured and not faster (4,001 x 5,120
 // x 17,408, beside this form's 390 us): pairs of CTAs on 256 x 256 tiles (cta_group::2)
 // 410-460, sixteen summing warps 400, halves of the weight rows handed over separately
 // 410, registers moved to the summing warps for two chunks in flight 410-450, rows of

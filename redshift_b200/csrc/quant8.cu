@@ -235,7 +235,7 @@ __device__ __forceinline__ void store_codes(const Norm8Params &p, int token, int
 // One CTA per row.  A warp takes every (warps)-th block of 128 columns, up to
 // PER_WARP of them in registers, so the row is read once, its sum of squares
 // meets in shared memory, and a block's maximum is a reduction inside one warp.
-// 4,096 rows x 5,120 with a residual: 45 us (272 MB, 6.0 TB/s); one row 3.6 us.
+// 4,096 rows x 5,120 with a residual: 45 us (272 MB, 6.0 TB/s); one row 3.4 us.
 constexpr int PER_WARP = 5, MAX_WARPS = 28;   // 140 blocks: 17,920 columns
 // The row's sum of all lanes' values (`red`: one float of each warp).
 __device__ __forceinline__ float row_sum(float *red, float v, int warp, int lane, int warps) {
