@@ -32,6 +32,7 @@ namespace {
 
 constexpr int KB = 128;                        // columns of a block = one 128-byte swizzled row of codes
 constexpr int ROWS = 128;                      // weight rows that share a scale
+constexpr int MAX_SPLITS = 6;                  // CTAs of a few_kernel cluster
 
 // D[tmem] (+)= A[smem] * B[smem]^T for e4m3 codes, fp32 accumulate, K = 32;
 // issued by a whole warp, one elected lane (see mma_f16_ts_by).
@@ -281,13 +282,13 @@ few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUte
         const bool vec = p.rows % 4 == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15) == 0;
         const uint32_t mine = smem_addr(part) + 16 * lane;
         for (int t = split + p.splits * (warp - 2); fine && t < live; t += p.splits * L::SUM_WARPS) {
-            float4 v[8];
+            float4 v[MAX_SPLITS];
 #pragma unroll
-            for (int q = 0; q < 8; ++q)
+            for (int q = 0; q < MAX_SPLITS; ++q)
                 if (q < p.splits) v[q] = ld_cluster_f32x4(cluster_rank(mine + t * ROWS * 4, q));
             float4 sum = v[0];
 #pragma unroll
-            for (int q = 1; q < 8; ++q)
+            for (int q = 1; q < MAX_SPLITS; ++q)
                 if (q < p.splits) { sum.x += v[q].x; sum.y += v[q].y; sum.z += v[q].z; sum.w += v[q].w; }
             float *dst = p.out + (size_t)(t0 + t) * p.rows + row4;
             if (vec) {
@@ -563,7 +564,7 @@ template <int NT> void launch_few(Mm8Params p, const void *weights, const void *
     // 6,144 x 5,120: four 9.6, six 10.0, seven 16.3, eight 15.6 us; 64 x 5,120 x
     // 10,240: two 17.6, three 15.6; 100 x 5,120 x 5,120: two 16.0, three 13.7).
     const long long slots = 148LL * L::CTAS, tiles = (long long)row_tiles * token_tiles;
-    const int splits = (int)std::max(1LL, std::min<long long>({6, slots / tiles, p.blocks / 4}));
+    const int splits = (int)std::max(1LL, std::min<long long>({MAX_SPLITS, slots / tiles, p.blocks / 4}));
     p.splits = splits;
     const CUtensorMap mw = codes_map(weights, width, p.rows, ROWS), mx = codes_map(x, width, p.tokens, NT);
     launch_cluster(few_kernel<NT>, dim3(splits, row_tiles, token_tiles), L::THREADS, L::SMEM, splits, st, mw, mx, p);
