@@ -56,6 +56,10 @@ __device__ __forceinline__ void copy_float(float *dst, const float *src, bool li
 __device__ __forceinline__ void arrive_copies(uint64_t *bar) {
     asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" :: "r"(smem_addr(bar)) : "memory");
 }
+// The box of `map` at (x, y) on its way into L2.
+__device__ __forceinline__ void prefetch_l2_2d(const CUtensorMap *map, int x, int y) {
+    asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" :: "l"(map), "r"(x), "r"(y) : "memory");
+}
 __device__ __forceinline__ bool warp_wait8(uint64_t *bar, uint32_t parity, volatile int *abort_flag) {
     return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag));
 }
@@ -135,6 +139,12 @@ few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUte
         fence_barrier_init();
         prefetch_tmap(&tmW);
         prefetch_tmap(&tmX);
+        // The ring's first weights, while the kernel before still runs: into L2, where
+        // what that kernel may yet write to them arrives too (behind a norm8, 8 x 5,120 x
+        // 17,408: 22.4 -> 21.1 us for both, 1 x 5,120 x 6,144: 17.9 -> 16.8; with the
+        // CTA's whole share asked for, 23.6 and 17.1).
+        if (!bad_base)
+            for (int j = 0; j < min(n, L::STAGES); ++j) prefetch_l2_2d(&tmW, (b0 + j) * KB, rtile * ROWS);
     }
     if (warp == 1) { tmem_alloc(tmem_slot, L::BUFS * NT); tmem_relinquish(); }
     tc_fence_before();
