@@ -211,12 +211,23 @@ __global__ void __launch_bounds__(THREADS8, 1) attention8_kernel(const FaParams 
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
+    // A converter warp's quarter of the tiles.  The first ones are asked for into L2 while
+    // the kernel before still runs; what it may yet write to them arrives there too
+    // (behind a norm8, 5 tokens at 32,767: 31.5 -> 30.0 us for both).
+    const int code_tiles = max(0, min(ntiles, c.blocks - tile0));       // tiles of codes, the first of this CTA's
+    const bool converts = warp >= SOFT_WARPS && warp < MMA_WARP;
+    const size_t step = (size_t)NKV * CODES_TILE;
+    const int8_t *codes = ((warp - SOFT_WARPS) >> 2 ? c.vc : c.kc) + ((size_t)tile0 * NKV + kv_head) * CODES_TILE + WARP_ROWS * (warp & 3) * HD;
+    auto prefetch = [&](int j) {
+        if (lane == 0 && j < code_tiles) prefetch_l2_bulk(codes + j * step, WARP_ROWS * HD);
+    };
+    if (converts)
+        for (int i = 0; i < AHEAD; ++i) prefetch(i);
     grid_dependency_wait();
     if (threadIdx.x == 0) launch_dependents();
 
-    const int code_tiles = max(0, min(ntiles, c.blocks - tile0));       // tiles of codes, the first of this CTA's
 
-    if (warp >= SOFT_WARPS && warp < MMA_WARP) {
+    if (converts) {
         // ------------------------------------------------ converters (warps 8-11: K, 12-15: V)
         // A lane takes 16 codes (16 dims of a row) at a time: 16 bytes of the
         // block, two 16-byte chunks of a 64-dim box of the image.  Eight
@@ -227,11 +238,6 @@ __global__ void __launch_bounds__(THREADS8, 1) attention8_kernel(const FaParams 
         const int part = (warp - SOFT_WARPS) >> 2, w = warp & 3, q = lane & 3, odd = lane >> 2 & 1;
         const int box = (lane >> 3) ^ odd, piece = 4 * box + q, row0 = WARP_ROWS * w + odd;
         const uint32_t image = box * (BN * 128) + row0 * 128;
-        const int8_t *codes = (part ? c.vc : c.kc) + ((size_t)tile0 * NKV + kv_head) * CODES_TILE + WARP_ROWS * w * HD;
-        const size_t step = (size_t)NKV * CODES_TILE;
-        auto prefetch = [&](int j) {
-            if (lane == 0 && j < code_tiles) prefetch_l2_bulk(codes + j * step, WARP_ROWS * HD);
-        };
         uint4 x[8];
         auto load = [&](int j) {
             const int8_t *src = codes + j * step + odd * HD + piece * 16;
@@ -279,10 +285,9 @@ __global__ void __launch_bounds__(THREADS8, 1) attention8_kernel(const FaParams 
         }
         uint64_t *full = part ? v_full : k_full, *empty = part ? v_empty : k_empty;
         const __half *rows = part ? p.vc : p.kc;
-        // The first tiles are asked for once the query rows have arrived, which would
-        // wait behind them.
+        // The first tile is asked for once the query rows have arrived, which would
+        // wait behind it.
         if (!warp_wait(q_loaded, 0, abort_flag)) return;
-        for (int i = 1; i < AHEAD; ++i) prefetch(i);
         if (code_tiles > 0) load(0);
         for (int j = 0; j < ntiles; ++j) {
             const int s = j & 1;
