@@ -11,7 +11,7 @@
 // scores and one of its probabilities.
 //
 // The floor is the cache's bytes, 2 KB a position: 8 tokens at 139,256 take 73 us
-// (3.9 TB/s, 375 TFLOP/s of products, 44 us at the copy rate), 5 at 32,767 28 us, 1
+// (3.9 TB/s, 375 TFLOP/s of products, 44 us at the copy rate), 5 at 32,767 27 us, 1
 // at 777 12 us; the fp16 cache's kernel takes 101 us for the longest.  What bounds
 // it is what a tile moves through shared memory (fp16 images written 64 KB and
 // read 64 KB by the MMAs, codes 32 KB: half as much again, and 3 % slower, when the

@@ -11,7 +11,7 @@
 // Two kernels:
 //  * few_kernel<NT> (tokens as the MMA's N, 16..128 of them): 128 weight rows
 //    per CTA.  Bound by reading the weights once from HBM (8 tokens x 5,120 x
-//    17,408: 18 us, 5.0 TB/s; 1 x 6,144 x 5,120, 31 MB, 9.6 us); the width is split
+//    17,408: 17.5 us, 5.1 TB/s; 1 x 6,144 x 5,120, 31 MB, 9.7 us); the width is split
 //    over a cluster of up to six CTAs whose partial sums meet in distributed
 //    shared memory in a fixed order, so that also few rows fill the SMs and no
 //    workspace or atomics are needed.
