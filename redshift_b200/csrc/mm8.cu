@@ -80,7 +80,10 @@ __device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr) {
                  : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
     return v;
 }
+// Every lane of the cluster's CTAs.  The aligned form wants a warp's lanes together, and
+// the code before it branches on the lane.
 __device__ __forceinline__ void cluster_sync() {
+    __syncwarp();
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
