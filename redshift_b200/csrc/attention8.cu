@@ -490,6 +490,7 @@ __global__ void __launch_bounds__(THREADS8, 1) attention8_kernel(const FaParams 
                 shift[u] = make_float2(f, f);
                 sum[u] = make_float2(0.f, 0.f);
             }
+            __syncwarp();                                          // all lanes store to TMEM together
 #pragma unroll
             for (int part = 0; part < 2; ++part) {
                 uint32_t hi[8], lo[8];

@@ -165,7 +165,9 @@ __device__ __forceinline__ void launch_dependents() {
 }
 
 // Named barrier over a subset of the CTA's warps (ids 1..15; 0 is __syncthreads).
+// bar.sync is the aligned form: a warp's lanes meet before it.
 __device__ __forceinline__ void named_barrier(uint32_t id, uint32_t threads) {
+    __syncwarp();
     asm volatile("bar.sync %0, %1;" :: "r"(id), "r"(threads) : "memory");
 }
 
