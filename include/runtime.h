@@ -333,7 +333,9 @@ int qv_quantize8(void *codes, float *scales, const float *x, int tokens, int wid
 
 /* out [tokens][rows] (fp32) = X W^T for e4m3 codes: weights [rows][width] with
  * fp32 weight_scales [ceil(rows/128)][ceil(width/128)] (one for every block of
- * 128 x 128), codes [tokens][width] with scales as above.  Any fp32 scales.
+ * 128 x 128), codes [tokens][width] with scales as above.  Any fp32 scales; outputs
+ * with a product of scales that is infinite or subnormal though neither scale is zero or
+ * infinite are computed anew, up to some hundred times slower.
  * width a multiple of 16 up to 65536, 1..248320 rows, tokens 1..139264;
  * weights and codes 16-byte aligned. */
 int qv_mm8(float *out, const void *weights, const float *weight_scales,

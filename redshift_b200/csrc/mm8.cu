@@ -4,9 +4,11 @@
 // for weights W [rows][width], activations X [tokens][width] and fp32 scales.
 //
 // Every block's sum of 128 products leaves the tensor core as fp32 and is
-// multiplied by its two scales and added in fp32 registers, so the scales may
-// be any fp32 values and a long width costs no precision (the products of one
-// block are exact in the accumulator's alignment for codes of like size).
+// multiplied by the product of its two scales and added in fp32 registers, so a long
+// width costs no precision (the products of one block are exact in the accumulator's
+// alignment for codes of like size).  The scales may be any fp32 values: outputs
+// with a product of scales that leaves fp32's normal range are computed anew
+// (again_in_range).
 //
 // Two kernels:
 //  * few_kernel<NT> (tokens as the MMA's N, 16..128 of them): 128 weight rows
@@ -63,6 +65,17 @@ __device__ __forceinline__ void prefetch_l2_2d(const CUtensorMap *map, int x, in
 __device__ __forceinline__ bool warp_wait8(uint64_t *bar, uint32_t parity, volatile int *abort_flag) {
     return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag));
 }
+// The values of four e4m3 codes.
+__device__ __forceinline__ void e4m3_values(uint32_t codes, float (&v)[4]) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        uint32_t h;
+        asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((unsigned short)(codes >> (16 * i))));
+        const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&h));
+        v[2 * i] = f.x;
+        v[2 * i + 1] = f.y;
+    }
+}
 __device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
     float v;
     asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
@@ -90,10 +103,93 @@ __device__ __forceinline__ void cluster_sync() {
 struct Mm8Params {
     float *out;
     const float *weight_scales, *scales;
-    int tokens, rows, blocks;                  // blocks = ceil(width / 128)
+    const uint8_t *weights, *codes;
+    int tokens, rows, width, blocks;           // blocks = ceil(width / 128)
     int splits;                                // cluster size (few_kernel)
     int m_tiles, tiles;                        // many_kernel: token tiles, all tiles
 };
+
+// ---------------------------------------------------------------- scales whose product leaves fp32
+// A product a b that is infinite or below 2^-126 although a and b are neither.
+__device__ __forceinline__ bool leaves_range(float a, float b) {
+    const float size = fabsf(a * b);
+    return !(size >= 0x1p-126f && size < INFINITY) && a != 0.f && b != 0.f && fabsf(a) < INFINITY && fabsf(b) < INFINITY;
+}
+// The range of scales that were looked at, zeros apart: bit patterns without the sign,
+// times two.  Two scales inside [2^-63, 2^63) have a normal product.
+struct ScaleRange {
+    uint32_t most = 0u, least = 0xFFFFFFFFu;                 // the largest; the smallest, less one, so that zero is the largest of all
+    __device__ __forceinline__ void add(float a) {
+        const uint32_t size = 2u * __float_as_uint(a);
+        most = max(most, size);
+        least = min(least, size - 1u);
+    }
+    __device__ __forceinline__ void add(float4 a) { add(a.x); add(a.y); add(a.z); add(a.w); }
+    __device__ __forceinline__ bool far() const { return most >= 2u * 0x5F000000u || least < 2u * 0x20000000u - 1u; }
+};
+// The outputs of `token` and the 128 rows of `row_block`, by one warp, if one of their
+// products of scales leaves fp32's normal range.  The factor a b of a block's sum S is
+// then g h with h a power of two, and S is multiplied by g first: S is zero or 2^-18 <=
+// |S| < 2^25, so S g is exact to a rounding, and only S g h, the term itself, may
+// leave fp32.  Such scales are rare: the warp that copies the scales only looks whether
+// any could be in such a product (ScaleRange), and this plain loop makes the outputs
+// good at the end of the kernel.  (Two steps in the summing loops took 3-25 % more of
+// every product, whichever warp looked for them; this takes 0-3 %, 0.3 us at most.)
+__device__ __forceinline__ void again_in_range(const Mm8Params &p, int token, int row_block) {
+    const int lane = threadIdx.x & 31;
+    const float *w_scales = p.weight_scales + (size_t)row_block * p.blocks;
+    bool leaves = false;
+    for (int b = lane; b < p.blocks; b += 32) leaves |= leaves_range(p.scales[(size_t)b * p.tokens + token], w_scales[b]);
+    if (!__any_sync(0xffffffffu, leaves)) return;
+    constexpr int AT_ONCE = 8;                                // rows on their way together
+    const int row0 = row_block * ROWS, row1 = min(row0 + ROWS, p.rows);
+    for (int row = row0; row < row1; row += AT_ONCE) {
+        float out[AT_ONCE] = {};
+        for (int b = 0; b < p.blocks; ++b) {
+            const int c = b * KB + 4 * lane;                  // this lane's columns of the block
+            const float s = p.scales[(size_t)b * p.tokens + token], v = w_scales[b];
+            uint32_t xc = 0u, wc[AT_ONCE] = {};
+            if (c < p.width) {
+                xc = *reinterpret_cast<const uint32_t *>(p.codes + (size_t)token * p.width + c);
+#pragma unroll
+                for (int i = 0; i < AT_ONCE; ++i)
+                    wc[i] = *reinterpret_cast<const uint32_t *>(p.weights + (size_t)min(row + i, row1 - 1) * p.width + c);
+            }
+            float x[4], w[4], sum[AT_ONCE];
+            e4m3_values(xc, x);
+#pragma unroll
+            for (int i = 0; i < AT_ONCE; ++i) {
+                e4m3_values(wc[i], w);
+                sum[i] = (w[0] * x[0] + w[1] * x[1]) + (w[2] * x[2] + w[3] * x[3]);
+            }
+#pragma unroll
+            for (int o = 16; o; o >>= 1)
+#pragma unroll
+                for (int i = 0; i < AT_ONCE; ++i) sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], o);
+            float g = 1.f, h = s * v;
+            if (leaves_range(s, v)) {
+                if (fabsf(h) < 1.f) {                         // neither is above 2^23; a term of a g below 2^-126 is below 2^-200
+                    g = (s * 0x1p50f) * (v * 0x1p50f);
+                    h = 0x1p-100f;
+                } else {                                      // both are above 1; a g of 2^100 is infinity for every sum but zero
+                    g = (s * 0x1p-64f) * (v * 0x1p-63f);
+                    g = copysignf(fminf(fabsf(g), 0x1p100f), g);
+                    h = 0x1p127f;
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < AT_ONCE; ++i) out[i] = fmaf(sum[i] * g, h, out[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; ++i)
+            if (lane == 0 && row + i < row1) p.out[(size_t)token * p.rows + row + i] = out[i];
+    }
+}
+
+// Tokens first, first + step, ... below `end`, by all warps of the CTA.
+__device__ __noinline__ void few_again(Mm8Params p, int first, int step, int end, int row_block) {
+    for (int t = first + step * (threadIdx.x >> 5); t < end; t += step * (blockDim.x >> 5)) again_in_range(p, t, row_block);
+}
 
 // ---------------------------------------------------------------- few tokens
 template <int NT> struct Few {
@@ -111,7 +207,7 @@ template <int NT> struct Few {
     static constexpr int SM_BAR = SM_SCALE + SLOTS * SLOT_FLOATS * 4;
     static constexpr int SMEM = SM_BAR + 384;
     static_assert(NT * ROWS * 4 <= STAGES * STAGE, "partial sums exceed the ring");
-    static_assert((2 * STAGES + 2 * BUFS + 2 * SLOTS + 1) * 8 + 8 <= 384, "barrier area");
+    static_assert((2 * STAGES + 2 * BUFS + 2 * SLOTS + 1) * 8 + 12 <= 384, "barrier area");
 };
 
 template <int NT>
@@ -123,7 +219,7 @@ few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUte
     uint64_t *d_full = empty + L::STAGES, *d_empty = d_full + L::BUFS, *s_full = d_empty + L::BUFS;
     uint64_t *s_empty = s_full + L::SLOTS, *mma_done = s_empty + L::SLOTS;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(mma_done + 1);
-    volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1), *far_flag = abort_flag + 1;
     float *slots = reinterpret_cast<float *>(smem + L::SM_SCALE);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -138,6 +234,7 @@ few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUte
         for (int i = 0; i < L::SLOTS; ++i) { mbar_init(s_full + i, 32); mbar_init(s_empty + i, L::SUM_WARPS); }
         mbar_init(mma_done, 1);
         *abort_flag = bad_base ? 1 : 0;
+        *far_flag = 0;
         if (bad_base) raise_status(STATUS_BAD_ARGUMENT);
         fence_barrier_init();
         prefetch_tmap(&tmW);
@@ -195,11 +292,18 @@ few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUte
             live[i] = t < NT && t0 + t < p.tokens;
             src[i] = p.scales + (size_t)b0 * p.tokens + (live[i] ? t0 + t : 0);
         }
+        ScaleRange range;
+        auto look_at = [&](const float *d) {
+            range.add(*reinterpret_cast<const float4 *>(d + 4 * lane % NT));
+            range.add(d[NT]);
+            __syncwarp();
+        };
         for (int j = 0, slot = 0, lap = 0; j < n; ++j) {
             // A slot has barriers of its own: `empty` may go on by two phases while
             // this warp is late, and its parity would then seem not to have changed.
             if (lap > 0 && !warp_wait8(s_empty + slot, (lap - 1) & 1, abort_flag)) { ok = false; break; }
             float *d = slots + slot * L::SLOT_FLOATS;
+            if (lap > 0) look_at(d);
 #pragma unroll
             for (int i = 0; i < PER_LANE; ++i) {
                 if (32 * i + lane < NT) copy_float(d + 32 * i + lane, src[i], live[i]);
@@ -210,6 +314,9 @@ few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUte
             if (++slot == L::SLOTS) { slot = 0; ++lap; }
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
+        __syncwarp();
+        for (int slot = 0; slot < min(n, L::SLOTS) && ok; ++slot) look_at(slots + slot * L::SLOT_FLOATS);
+        if (range.far()) *far_flag = 1;
     } else if (warp == 1) {
         // ------------------------------------------------ MMA issuer
         constexpr uint32_t idesc = idesc_e4m3(ROWS, NT);
@@ -273,6 +380,10 @@ few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUte
             for (int t = 0; t < L::COLS; ++t)
                 if (col0 + t < live) p.out[(size_t)(t0 + col0 + t) * p.rows + row] = t & 1 ? acc[t / 2].y : acc[t / 2].x;
         }
+        if (*far_flag && all_ok) {
+            __syncthreads();
+            few_again(p, t0, 1, t0 + live, rtile);
+        }
         return;
     }
     // Partial sums of the splits meet in shared memory (the idle ring); CTA q
@@ -287,6 +398,8 @@ few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUte
     }
     if (threadIdx.x == 0) *good = all_ok;
     cluster_sync();
+    if (threadIdx.x == 0 && *far_flag)                        // every CTA of the cluster has outputs of this one's blocks
+        for (int q = 0; q < p.splits; ++q) st_cluster_f32(cluster_map(const_cast<int *>(far_flag), q), 1.f);
     if (sums) {
         bool fine = true;
         for (int q = 0; q < p.splits; ++q) fine = fine && __float_as_int(ld_cluster_f32(cluster_map(good, q))) != 0;
@@ -315,6 +428,7 @@ few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUte
         }
     }
     cluster_sync();
+    if (*far_flag) few_again(p, t0 + split, p.splits, min(t0 + NT, p.tokens), rtile);
 }
 
 // ---------------------------------------------------------------- many tokens
@@ -340,6 +454,16 @@ struct Many {
     static_assert(SMEM <= 227 * 1024, "shared memory of a CTA");
 };
 
+// again_in_range over the tiles of this CTA; apart, so that nothing has to be kept for it.
+__device__ __noinline__ void many_again(Mm8Params p) {
+    const int row_blocks = (p.rows + ROWS - 1) / ROWS;
+    for (int tile = blockIdx.x; tile < p.tiles; tile += gridDim.x) {
+        const int m0 = tile % p.m_tiles * Many::MT, r0 = tile / p.m_tiles * (Many::NT / ROWS);
+        for (int q = threadIdx.x >> 5; q < 2 * min(Many::MT, p.tokens - m0); q += Many::THREADS / 32)
+            if (r0 + (q & 1) < row_blocks) again_in_range(p, m0 + (q >> 1), r0 + (q & 1));
+    }
+}
+
 __global__ void __launch_bounds__(Many::THREADS, 1)
 many_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX, const Mm8Params p) {
     using L = Many;
@@ -348,7 +472,7 @@ many_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUt
     uint64_t *d_full = empty + L::STAGES, *d_empty = d_full + L::BUFS, *s_full = d_empty + L::BUFS;
     uint64_t *s_empty = s_full + L::SLOTS, *mma_done = s_empty + L::SLOTS;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(mma_done + 1);
-    volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1), *far_flag = abort_flag + 1;
     float *slots = reinterpret_cast<float *>(smem + L::SM_SCALE);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -359,6 +483,7 @@ many_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUt
         for (int i = 0; i < L::SLOTS; ++i) { mbar_init(s_full + i, 32); mbar_init(s_empty + i, L::SUM_WARPS); }
         mbar_init(mma_done, 1);
         *abort_flag = bad_base ? 1 : 0;
+        *far_flag = 0;
         if (bad_base) raise_status(STATUS_BAD_ARGUMENT);
         fence_barrier_init();
         prefetch_tmap(&tmW);
@@ -406,6 +531,12 @@ many_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUt
         // ------------------------------------------------ scales, by small copies
         int slot = 0, lap = 0;
         bool ok = true;
+        ScaleRange range;
+        auto look_at = [&](const float *d) {
+            range.add(*reinterpret_cast<const float4 *>(d + 4 * lane));
+            range.add(d[L::MT + (lane & 1)]);
+            __syncwarp();
+        };
         for (int i = 0; i < mine && ok; ++i) {
             const int tile = blockIdx.x + i * gridDim.x, m0 = tile % p.m_tiles * L::MT, n0 = tile / p.m_tiles * L::NT;
             bool live[4];
@@ -420,6 +551,7 @@ many_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUt
             for (int b = 0; b < p.blocks; ++b) {
                 if (lap > 0 && !warp_wait8(s_empty + slot, (lap - 1) & 1, abort_flag)) { ok = false; break; }
                 float *d = slots + slot * L::SLOT_FLOATS;
+                if (lap > 0) look_at(d);
 #pragma unroll
                 for (int t = 0; t < 4; ++t) {
                     copy_float(d + 32 * t + lane, src[t], live[t]);
@@ -431,6 +563,9 @@ many_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUt
             }
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
+        __syncwarp();
+        for (int q = 0; q < min(mine * p.blocks, L::SLOTS) && ok; ++q) look_at(slots + q * L::SLOT_FLOATS);
+        if (range.far()) *far_flag = 1;
     } else if (warp == 1) {
         constexpr uint32_t idesc = idesc_e4m3(L::MT, L::NT);
         const uint32_t lead = elect_lane(), tm = __shfl_sync(0xffffffffu, tmem, 0);
@@ -525,6 +660,7 @@ many_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUt
     __syncthreads();
     tc_fence_after();
     if (warp == 1) tmem_dealloc(tmem, 512);
+    if (*far_flag && !*abort_flag) many_again(p);
 }
 
 // ---------------------------------------------------------------- host
@@ -592,7 +728,8 @@ void mm8(float *out, const void *weights, const float *weight_scales, const void
         reserve(few_kernel<64>, Few<64>::SMEM); reserve(few_kernel<128>, Few<128>::SMEM);
         reserve(many_kernel, Many::SMEM);
     });
-    Mm8Params p{out, weight_scales, scales, tokens, rows, (width + KB - 1) / KB, 1, 0, 0};
+    Mm8Params p{out, weight_scales, scales, static_cast<const uint8_t *>(weights), static_cast<const uint8_t *>(x),
+                tokens, rows, width, (width + KB - 1) / KB, 1, 0, 0};
     const int m_tiles = (tokens + Many::MT - 1) / Many::MT;
     const long long tiles = (long long)m_tiles * ((rows + Many::NT - 1) / Many::NT);
     // Beyond 128 tokens few_kernel<128> is still the faster one while all its tiles
