@@ -40,7 +40,9 @@ class Cache8:
         return self.key_codes, self.key_scales, self.value_codes, self.value_scales
 
     def pack(self, position):
-        """Pack the blocks that are complete before `position`."""
+        """Pack the blocks that are complete before `position`, a number of kept tokens."""
+        if not 0 <= position <= self.rows:
+            raise ValueError(f'position {position} cannot be packed: the cache holds {self.rows} rows')
         end = position // BLOCK * BLOCK
         if end > self.packed:
             if self.hot.capturing():

@@ -1,0 +1,40 @@
+"""What Cache8 counts on the host: positions packed, positions that hold a row.  No GPU: the calls are recorded."""
+import pytest
+
+from redshift_b200 import Cache8
+
+
+class Recorder:
+    """Stands for HotPath: notes the calls; `capture` says whether the stream of a device is being captured."""
+
+    def __init__(self, capture=False):
+        self.calls, self.capture = [], capture
+
+    def capturing(self, *device):
+        return self.capture
+
+    def __getattr__(self, name):
+        return lambda *args: self.calls.append(name)
+
+
+def _cache(context=256, **kw):
+    return Cache8(Recorder(**kw), context, device='cpu:0')
+
+
+def _step(cache, batch, position):
+    cache.attention(None, None, None, None, None, None, batch, position)
+
+
+@pytest.mark.parametrize('position', [71, 128, -1, 257])
+def test_rows_that_are_not_there_are_not_packed(position):
+    """Rows behind the last one are stale or were never written."""
+    cache = _cache()
+    for at in range(0, 70, 10):
+        _step(cache, 10, at)
+    before = len(cache.hot.calls), cache.packed, cache.rows
+    with pytest.raises(ValueError, match='70 rows'):
+        cache.pack(position)
+    assert (len(cache.hot.calls), cache.packed, cache.rows) == before
+    cache.pack(70)
+    assert cache.packed == 64
+    _step(cache, 1, 70)
