@@ -9,8 +9,10 @@
 
 ``position`` is the caller's count of kept tokens: after a verify of 8 tokens of which 3 were kept
 the next call simply passes a position that is 3 higher.  Rows from ``position`` on are never
-packed, so nothing has to be rolled back.  The host keeps count of what is packed: a captured
-graph replays one position only, so capture ``HotPath.attention8`` itself where that is wanted.
+packed, so nothing has to be rolled back.  The host keeps count of the rows and of what is packed, so
+``attention``, ``pack`` and ``load`` are refused under graph capture: a replay would write the tail rows
+of one position again, which hold others once the ring has gone on.  Capture ``HotPath.attention8``
+itself where one position is to be replayed.
 """
 BLOCK = 64
 
@@ -36,6 +38,10 @@ class Cache8:
         self.packed = 0                  # positions in the packed part
         self.rows = 0                    # positions that hold a row
 
+    def _not_captured(self):
+        if self.hot.capturing():
+            raise RuntimeError('the cache cannot be changed under graph capture: a replay would write rows that have gone on')
+
     def _packed_buffers(self):
         return self.key_codes, self.key_scales, self.value_codes, self.value_scales
 
@@ -45,8 +51,7 @@ class Cache8:
             raise ValueError(f'position {position} cannot be packed: the cache holds {self.rows} rows')
         end = position // BLOCK * BLOCK
         if end > self.packed:
-            if self.hot.capturing():
-                raise RuntimeError('blocks cannot be packed under graph capture: a replay would pack rows that have gone on')
+            self._not_captured()
             self.hot.cache8_pack(*self._packed_buffers(), self.key_tail, self.value_tail, self.packed, end)
             self.packed = end
 
@@ -55,6 +60,7 @@ class Cache8:
         the rest into the tail."""
         if not 0 <= rows <= min(self.context, key_rows.shape[0], value_rows.shape[0]):
             raise ValueError('rows exceed the context or the given cache')
+        self._not_captured()
         end = rows // BLOCK * BLOCK
         self.hot.cache8_pack(*self._packed_buffers(), key_rows, value_rows, 0, end)
         if rows > end:
@@ -81,6 +87,7 @@ class Cache8:
             raise ValueError(f'the cache holds {self.context} positions')
         if position > self.rows:
             raise ValueError(f'position {position} leaves a gap: the cache holds {self.rows} rows')
+        self._not_captured()
         self.pack(position)
         self.hot.attention8(out, *self._packed_buffers(), self.packed, self.key_tail, self.value_tail, q_gate, key,
                             value, q_norm, k_norm, batch, position, epsilon, workspace)

@@ -38,3 +38,23 @@ def test_rows_that_are_not_there_are_not_packed(position):
     cache.pack(70)
     assert cache.packed == 64
     _step(cache, 1, 70)
+
+
+def test_nothing_is_counted_under_capture():
+    """A captured call writes no row yet, and its replays would write the tail rows of one position, which hold
+    others once the ring has gone on."""
+    import torch
+    cache = _cache()
+    _step(cache, 10, 0)
+    cache.hot.capture = True
+    rows = torch.zeros((200, 4, 256), dtype=torch.float16)
+    for call in (lambda: _step(cache, 1, 10), lambda: cache.load(rows, rows, 130)):
+        with pytest.raises(RuntimeError, match='capture'):
+            call()
+    assert (cache.packed, cache.rows) == (0, 10) and cache.hot.calls == ['attention8']
+    cache.hot.capture = False
+    with pytest.raises(ValueError, match='leaves a gap'):
+        _step(cache, 1, 11)
+    _step(cache, 1, 10)
+    cache.load(rows, rows, 130)
+    assert (cache.packed, cache.rows) == (128, 130)
