@@ -39,7 +39,7 @@ class Cache8:
         self.rows = 0                    # positions that hold a row
 
     def _not_captured(self):
-        if self.hot.capturing():
+        if self.hot.capturing(self.key_codes.device):
             raise RuntimeError('the cache cannot be changed under graph capture: a replay would write rows that have gone on')
 
     def _packed_buffers(self):

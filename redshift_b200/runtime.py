@@ -159,10 +159,13 @@ class HotPath:
         return ct.c_void_p(torch.cuda.current_stream().cuda_stream)
 
     @staticmethod
-    def capturing():
-        """Whether torch's current stream is being captured into a graph."""
+    def capturing(device=None):
+        """Whether torch's current stream of `device` (of the current device) is being captured into a graph."""
         import torch
-        return torch.cuda.is_current_stream_capturing()
+        if device is None or getattr(device, 'index', device) == torch._C._cuda_getDevice():
+            return torch.cuda.is_current_stream_capturing()
+        with torch.cuda.device(device):
+            return torch.cuda.is_current_stream_capturing()
 
     @staticmethod
     def _ptr(t):
@@ -373,7 +376,7 @@ class HotPath:
         need_tensor(value_tail, types.half, (tail, 4, 256), 'value_tail', dev)
         need_cache8(types, key_codes, key_scales, value_codes, value_scales, packed, dev)
         if workspace is None:
-            if self.capturing():
+            if self.capturing(dev):
                 raise ValueError('attention8 under graph capture needs a workspace of its own (attention8_workspace)')
             which = (dev, torch._C._cuda_getCurrentRawStream(dev))
             workspace = self._workspaces8.get(which)

@@ -58,3 +58,33 @@ def test_nothing_is_counted_under_capture():
     _step(cache, 1, 10)
     cache.load(rows, rows, 130)
     assert (cache.packed, cache.rows) == (128, 130)
+
+
+def test_capture_is_looked_for_on_the_device_of_the_tensors(monkeypatch):
+    """The calls run on the current stream of the tensors' device, whichever device is current."""
+    import torch
+    from redshift_b200 import HotPath
+    current = [0]
+
+    class Current:
+        def __init__(self, device):
+            self.device = device
+
+        def __enter__(self):
+            self.before, current[0] = current[0], torch.device('cuda', self.device).index if isinstance(self.device, int) else self.device.index
+
+        def __exit__(self, *_):
+            current[0] = self.before
+    monkeypatch.setattr(torch.cuda, 'device', Current)
+    monkeypatch.setattr(torch.cuda, 'is_current_stream_capturing', lambda: current[0] == 1)
+    monkeypatch.setattr(torch._C, '_cuda_getDevice', lambda: current[0], raising=False)
+    hot = object.__new__(HotPath)
+    assert hot.capturing(1) and hot.capturing(torch.device('cuda', 1))
+    assert not hot.capturing(0) and not hot.capturing()
+    current[0] = 1
+    assert not hot.capturing(0) and hot.capturing(1) and hot.capturing()
+    asked = []
+    cache = _cache()
+    cache.hot.capturing = lambda *device: asked.append(device)
+    _step(cache, 10, 0)
+    assert asked and all(device == (cache.key_codes.device,) for device in asked)
