@@ -358,12 +358,26 @@ class HotPath:
         ws[:256].zero_()
         return ws
 
+    KEPT_WORKSPACES8 = 16
+
+    def kept_workspace8(self, device):
+        """The workspace of the current stream of device number `device`.  The newest KEPT_WORKSPACES8 are kept
+        (10 MB each); an older one goes back to torch's allocator, which gives its memory to later work of the
+        same stream only."""
+        import torch
+        which = (device, torch._C._cuda_getCurrentRawStream(device))
+        workspace = self._workspaces8.get(which)
+        if workspace is None:
+            workspace = self._workspaces8[which] = self.attention8_workspace(torch.device('cuda', device))
+            while len(self._workspaces8) > self.KEPT_WORKSPACES8:
+                self._workspaces8.pop(next(iter(self._workspaces8)), None)
+        return workspace
+
     def attention8(self, out, key_codes, key_scales, value_codes, value_scales, packed, key_tail, value_tail, q_gate,
                    key, value, q_norm, k_norm, batch, position, epsilon=1e-6, workspace=None):
         """qv_attention8: one attention layer for 1..10 new tokens over the 8-bit cache's first `packed`
         positions and the fp16 tail.  Without `workspace`, one that is kept for the current stream is used;
         under graph capture it has to be given (attention8_workspace), since the graph goes on using it."""
-        import torch
         types = self._types
         dev, tail = out.get_device(), key_tail.shape[0]
         need_tensor(out, types.float, (batch, 24, 256), 'out', dev)
@@ -378,10 +392,7 @@ class HotPath:
         if workspace is None:
             if self.capturing(dev):
                 raise ValueError('attention8 under graph capture needs a workspace of its own (attention8_workspace)')
-            which = (dev, torch._C._cuda_getCurrentRawStream(dev))
-            workspace = self._workspaces8.get(which)
-            if workspace is None:
-                workspace = self._workspaces8[which] = self.attention8_workspace(out.device)
+            workspace = self.kept_workspace8(dev)
         else:
             need_tensor(workspace, types.bytes, workspace.shape, 'workspace', dev)
         self._call(dev, self.lib.qv_attention8, out.data_ptr(), key_codes.data_ptr(), key_scales.data_ptr(),
