@@ -61,7 +61,11 @@ class Cache8:
         if not 0 <= rows <= min(self.context, key_rows.shape[0], value_rows.shape[0]):
             raise ValueError('rows exceed the context or the given cache')
         self._not_captured()
+        if rows == 0:
+            self.packed = self.rows = 0
+            return
         end = rows // BLOCK * BLOCK
+        key_rows, value_rows = key_rows[:rows], value_rows[:rows]
         self.hot.cache8_pack(*self._packed_buffers(), key_rows, value_rows, 0, end)
         if rows > end:
             at = end % self.key_tail.shape[0]        # whole blocks: the rest does not wrap
@@ -73,11 +77,14 @@ class Cache8:
         """Write the first `position` positions as fp16 rows, e.g. to prefill a further block behind them."""
         if not self.packed <= position <= min(self.rows, key_rows.shape[0], value_rows.shape[0]):
             raise ValueError('position is outside the cache or the given rows')
+        if position == 0:
+            return
         import torch
+        key_rows, value_rows = key_rows[:position], value_rows[:position]
         self.hot.cache8_unpack(key_rows, value_rows, *self._packed_buffers(), 0, self.packed)
         tail = torch.arange(self.packed, position, device=self.key_tail.device) % self.key_tail.shape[0]
-        key_rows[self.packed:position] = self.key_tail[tail]
-        value_rows[self.packed:position] = self.value_tail[tail]
+        key_rows[self.packed:] = self.key_tail[tail]
+        value_rows[self.packed:] = self.value_tail[tail]
 
     def attention(self, out, q_gate, key, value, q_norm, k_norm, batch, position, epsilon=1e-6, workspace=None):
         """qv_attention8 for `batch` new tokens at `position`, after packing what is complete before it."""

@@ -88,3 +88,29 @@ def test_capture_is_looked_for_on_the_device_of_the_tensors(monkeypatch):
     cache.hot.capturing = lambda *device: asked.append(device)
     _step(cache, 10, 0)
     assert asked and all(device == (cache.key_codes.device,) for device in asked)
+
+
+def test_a_prefill_of_no_tokens_and_rows_of_two_lengths():
+    """`rows` may be anything up to the shorter buffer's length, zero with empty buffers among it."""
+    import torch
+    calls = []
+
+    class Shapes(Recorder):
+        def cache8_pack(self, *args):
+            calls.append([tuple(a.shape) for a in args[4:6]] + list(args[6:]))
+
+        def cache8_unpack(self, *args):
+            calls.append([tuple(a.shape) for a in args[:2]] + list(args[6:]))
+    cache = Cache8(Shapes(), 256, device='cpu:0')
+    none, short, long = (torch.zeros((n, 4, 256), dtype=torch.float16) for n in (0, 130, 200))
+    cache.load(none, none, 0)
+    cache.unload(none, none, 0)
+    assert calls == [] and (cache.packed, cache.rows) == (0, 0)
+    _step(cache, 10, 0)
+    cache.load(long, short, 130)
+    cache.unload(short, long, 130)
+    assert calls == [[(130, 4, 256), (130, 4, 256), 0, 128], [(130, 4, 256), (130, 4, 256), 0, 128]]
+    assert (cache.packed, cache.rows) == (128, 130)
+    cache.load(none, none, 0)                            # a new conversation
+    assert (cache.packed, cache.rows) == (0, 0)
+    _step(cache, 1, 0)
