@@ -244,11 +244,9 @@ __device__ __forceinline__ void mma_commit(uint64_t *bar) {
                  :: "r"(smem_addr(bar)) : "memory");
 }
 // Issue by a whole warp: every lane runs the same code with the same operands
-// and one elected lane executes the instruction.  The operands then stay in
-// uniform registers and an MMA costs the warp a few issue slots; issued from
-// inside `if (lane == 0)` each operand is moved there first, and beside busy
-// warps of the same scheduler a chain of 20 MMAs took 2,624 cycles instead of
-// 1,038 (measured with two warps of FMAs a scheduler).
+// and one elected lane executes the instruction.  Beside busy warps of the same
+// scheduler a chain of 20 MMAs took 1,038 cycles this way and 2,624 issued from
+// inside `if (lane == 0)` (measured with two warps of FMAs a scheduler).
 __device__ __forceinline__ uint32_t elect_lane() {
     uint32_t r;
     asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));

@@ -208,7 +208,8 @@ __device__ __forceinline__ void store_codes(const Norm8Params &p, int token, int
     if (finite && scale > 0.f) {
         float q[4];
         if (scale > 0x1p-100f) {
-            // the quotient from the reciprocal, with one correction by its remainder
+            // Markstein's division: the quotient from the correctly rounded reciprocal, corrected
+            // once by its exact remainder (P. Markstein, IBM J. Res. Dev. 34, 1990)
             const float inv = __frcp_rn(scale);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
