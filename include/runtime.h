@@ -323,7 +323,8 @@ int qv_attention_noalloc(float *out, void *key_cache, void *value_cache,
  * rsqrt(mean(s^2) + epsilon) * weights, codes and scales of y.  residual_out
  * (NULL: not written) receives s, normed (NULL: not written) y in fp32; either
  * may be x or residual itself, and they must not be the same buffer.
- * x, residual: [tokens][width]; weights: [width]; 1 <= width <= 17408.
+ * x, residual: [tokens][width]; weights: [width]; 1 <= width <= 17408; 1 <=
+ * tokens <= 139264 (qv_quantize8 too).
  * qv_quantize8: codes and scales of x itself. */
 int qv_norm8(void *codes, float *scales, float *residual_out, float *normed,
              const float *x, const float *residual, const float *weights,

@@ -20,7 +20,7 @@ CSRC = ROOT / 'redshift_b200' / 'csrc'
 BUILD = ROOT / 'build'
 LIBRARY = BUILD / 'libqvelox.so'
 SOURCES = ['status.cu', 'attention.cu', 'delta.cu', 'gdn_chunk.cu', 'delta_prefill.cu', 'prefill.cu', 'projection.cu', 'copy.cu',
-           'attention8.cu', 'quant8.cu', 'mm8.cu',           'runtime.cu', 'noalloc.cu']
+           'attention8.cu', 'quant8.cu', 'mm8.cu', 'runtime.cu', 'noalloc.cu']
 HEADERS = ['common.cuh', 'attention_core.cuh', 'hotpath.h']
 
 NVCC_FLAGS = [

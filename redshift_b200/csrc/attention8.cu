@@ -112,8 +112,7 @@ __device__ __forceinline__ uint4 fp16_codes(uint32_t a, uint32_t b) {
 // cache is read by every later token, so the keys are formed in 64 bits, and the
 // correctly rounded fp32 value goes to fp16 (formed in 32 bits, a value near a border
 // of two fp16 numbers now and then went to the further one); the warps are idle
-// meanwhile.  Returns the tokens, as
-// bits, whose fp16 values are not all finite.
+// meanwhile.  Returns the tokens, as bits, whose fp16 values are not all finite.
 __device__ __forceinline__ uint32_t append_row8(const FaParams &p, int ring, int kv_head, int pos, int end) {
     const int lane = threadIdx.x & 31;
     uint32_t bad = 0;
@@ -225,7 +224,6 @@ __global__ void __launch_bounds__(THREADS8, 1) attention8_kernel(const FaParams 
         for (int i = 0; i < AHEAD; ++i) prefetch(i);
     grid_dependency_wait();
     if (threadIdx.x == 0) launch_dependents();
-
 
     if (converts) {
         // ------------------------------------------------ converters (warps 8-11: K, 12-15: V)

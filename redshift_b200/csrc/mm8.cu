@@ -12,8 +12,9 @@
 //
 // Two kernels:
 //  * few_kernel<NT> (tokens as the MMA's N, 16..128 of them): 128 weight rows
-//    per CTA.  Bound by reading the weights once from HBM (8 tokens x 5,120 x
-//    17,408: 17.5 us, 5.1 TB/s; 1 x 6,144 x 5,120, 31 MB, 9.7 us); the width is split
+//    per CTA.  Up to 16 tokens bound by reading the weights once from HBM (8 tokens x
+//    5,120 x 17,408: 17.7 us, 5.0 TB/s; 1 x 6,144 x 5,120, 31 MB, 9.9 us), at 128 by the
+//    way of the sums out of TMEM (128 x 5,120 x 10,240: 24.0 us); the width is split
 //    over a cluster of up to six CTAs whose partial sums meet in distributed
 //    shared memory in a fixed order, so that also few rows fill the SMs and no
 //    workspace or atomics are needed.
@@ -21,7 +22,8 @@
 //    CTAs.  With tokens in the TMEM lanes the two scales of a thread's columns are
 //    one factor per block.  Bound by the way of a block's sums out of TMEM, see
 //    there (4,001 x 5,120 x 17,408: 368-410 us, up to 1.9 PFLOP/s; in calls without a
-//    pause the power limit holds the SMs at 1.3-1.5 GHz, 425-455 us).
+//    pause the power limit holds the SMs at 1.3-1.5 GHz, 425-455 us; 1,000 x 5,120 x
+//    10,240 71 us).
 #include "common.cuh"
 #include "hotpath.h"
 
@@ -711,7 +713,8 @@ template <int NT> void launch_few(Mm8Params p, const void *weights, const void *
     // Split the width as far as the CTAs fit the SMs at once and every CTA keeps four
     // blocks, but not over clusters of more than six: seven and eight pack badly (1 x
     // 6,144 x 5,120: four 9.6, six 10.0, seven 16.3, eight 15.6 us; 64 x 5,120 x
-    // 10,240: two 17.6, three 15.6; 100 x 5,120 x 5,120: two 16.0, three 13.7).
+    // 10,240: two 17.6, three 15.6; 100 x 5,120 x 5,120: two 16.0, three 13.4; all
+    // before far scales were looked for, which adds up to 0.3).
     const long long slots = 148LL * L::CTAS, tiles = (long long)row_tiles * token_tiles;
     const int splits = (int)std::max(1LL, std::min<long long>({MAX_SPLITS, slots / tiles, p.blocks / 4}));
     p.splits = splits;
@@ -733,7 +736,7 @@ void mm8(float *out, const void *weights, const float *weight_scales, const void
     const int m_tiles = (tokens + Many::MT - 1) / Many::MT;
     const long long tiles = (long long)m_tiles * ((rows + Many::NT - 1) / Many::NT);
     // Beyond 128 tokens few_kernel<128> is still the faster one while all its tiles
-    // run at once (384 x 5,120 x 5,120: 24.1 against 27.1 us, 256 x 17,408 x 5,120: 65
+    // run at once (384 x 5,120 x 5,120: 23.3 against 27.1 us, 256 x 17,408 x 5,120: 65
     // against 72; two waves of it, 256 x 5,120 x 10,240: 42 against 28).
     const long long few_tiles = (long long)((tokens + 127) / 128) * ((rows + ROWS - 1) / ROWS);
     if (tokens > 128 && few_tiles > 148) {
